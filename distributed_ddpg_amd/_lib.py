@@ -26,7 +26,8 @@ LIB_PATH = _ALT or os.path.join(_HERE, "libddpg_hip.so")
 
 DDPG_OK = 0
 DDPG_EINVAL, DDPG_EHIP, DDPG_ENOMEM, DDPG_ESTATE, DDPG_ECOMM = -1, -2, -3, -4, -5
-FP32, BF16 = 0, 1
+FP32, BF16, FP16 = 0, 1, 2
+ACT_NONE, ACT_ELU, ACT_TANH = 0, 1, 2
 ACTOR, ACTOR_TARGET, CRITIC, CRITIC_TARGET = 0, 1, 2, 3
 ACTOR_ADAM_M, ACTOR_ADAM_V, CRITIC_ADAM_M, CRITIC_ADAM_V = 4, 5, 6, 7
 ACTOR_GRAD, CRITIC_GRAD = 8, 9
@@ -72,6 +73,10 @@ _dp = ctypes.POINTER(ctypes.c_double)
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _u8p = ctypes.POINTER(ctypes.c_uint8)
 _u32p = ctypes.POINTER(ctypes.c_uint32)
+_ip = ctypes.POINTER(ctypes.c_int)
+_PP = ctypes.POINTER(ctypes.c_void_p)
+_szp = ctypes.POINTER(ctypes.c_size_t)
+_i64 = ctypes.c_int64
 
 # (name, restype, argtypes) -- must match include/ddpg_hip.h
 PROTOTYPES = [
@@ -121,6 +126,20 @@ PROTOTYPES = [
     ("ddpg_step_counts", _c.c_int, [_P, _i64p, _i64p, _c.POINTER(_c.c_int)]),
     ("ddpg_profile_enable", _c.c_int, [_P, _c.c_int]),
     ("ddpg_profile_read", _c.c_int, [_P, _c.c_int, _P, _dp, _i64p, _dp, _dp]),
+    ("ddpg_global_norm_workspace", _c.c_size_t, [_c.c_int]),
+    ("ddpg_global_norm", _c.c_int, [_c.c_int, _P, _c.c_int, _ip, _PP, _i64p, _i64p, _i64p, _P,
+                                    _c.c_size_t, _P]),
+    ("ddpg_clip_by_global_norm", _c.c_int, [_c.c_int, _P, _c.c_int, _ip, _PP, _PP, _i64p, _i64p,
+                                            _i64p, _c.c_float, _P, _P, _c.c_size_t, _P]),
+    ("ddpg_mx_sizes", _c.c_int, [_i64, _i64, _szp, _szp]),
+    ("ddpg_mx_quantize", _c.c_int, [_c.c_int, _P, _c.c_int, _P, _i64, _i64, _i64, _i64, _P, _P]),
+    ("ddpg_mx_dequantize", _c.c_int, [_c.c_int, _P, _P, _P, _i64, _i64, _c.c_int, _P, _i64]),
+    ("ddpg_mx_linear", _c.c_int, [_c.c_int, _P, _c.c_int, _P, _i64, _i64, _P, _P, _i64, _i64, _P,
+                                  _P, _i64, _c.c_int, _P, _c.c_int, _c.c_int, _P, _i64]),
+    ("ddpg_mx_linear_grad_workspace", _c.c_size_t, [_c.c_int, _i64, _i64, _i64, _c.c_int,
+                                                    _c.c_int, _c.c_int]),
+    ("ddpg_mx_linear_grad", _c.c_int, [_c.c_int, _P, _c.c_int, _P, _i64, _i64, _i64, _i64, _i64,
+                                       _P, _P, _P, _P, _P, _P, _P, _P, _c.c_size_t]),
     ("ddpg_crc32c", _c.c_uint32, [_c.c_uint32, _c.c_void_p, _c.c_size_t]),
 ]
 

@@ -46,7 +46,11 @@ enum ddpg_status {
   DDPG_ECOMM = -5     /* RCCL error */
 };
 
-enum ddpg_dtype { DDPG_FP32 = 0, DDPG_BF16 = 1 };
+/* a ctx is DDPG_FP32 or DDPG_BF16; the tensor operators take all three */
+enum ddpg_dtype { DDPG_FP32 = 0, DDPG_BF16 = 1, DDPG_FP16 = 2 };
+
+/* activation of ddpg_mx_linear: the networks' (networks.py:54-62) or none */
+enum ddpg_act { DDPG_ACT_NONE = 0, DDPG_ACT_ELU = 1, DDPG_ACT_TANH = 2 };
 
 /* which parameter set (ddpg_set_params / ddpg_get_params) */
 enum ddpg_which {
@@ -242,6 +246,67 @@ int ddpg_profile_enable(ddpg_ctx* ctx, int enable);
  * <=63 chars), total ms, launches and algorithmic flop / bytes. Returns count. */
 int ddpg_profile_read(ddpg_ctx* ctx, int n, char (*names)[64], double* ms, int64_t* launches,
                       double* flops, double* bytes);
+
+/* -------------------------------------------------------- tensor operators
+ * On the caller's device tensors, without a ctx: device pointers, a device
+ * ordinal and the HIP stream to launch on (NULL: the default stream).  Calls
+ * only launch (no synchronisation, no allocation, no state), so they may be
+ * captured into a graph and issued from any thread; outputs and workspaces are
+ * the caller's and must not be shared by calls that may run at once.  Errors as
+ * above, message in ddpg_global_error().  dtype: enum ddpg_dtype.
+ * distributed_ddpg_amd/ops.py is the Python form.
+ *
+ * A list of n tensors: dtype[i], a pointer, count[i] elements.  cols / ld
+ * (both NULL, or arrays): where cols[i] > 0 tensor i is rows of cols[i]
+ * adjacent elements, ld[i] elements apart; otherwise it is dense. */
+size_t ddpg_global_norm_workspace(int n);
+/* *norm = sqrt(sum of all squares) (tf.global_norm), summed in float64 in a
+ * fixed order.  ws: ddpg_global_norm_workspace(n) bytes, 8-byte aligned. */
+int ddpg_global_norm(int device, void* stream, int n, const int* dtype, const void* const* src,
+                     const int64_t* count, const int64_t* cols, const int64_t* ld, void* ws,
+                     size_t ws_bytes, float* norm);
+/* tf.clip_by_global_norm: dst = src * (norm <= clip_norm ? 1 : clip_norm /
+ * norm), norm written to *norm; use_norm (device, optional) instead of the
+ * list's own norm (ws and norm may then be NULL).  A NaN norm makes every
+ * result NaN, an infinite one every finite result 0 and the rest NaN.  dst[i]
+ * == src[i] clips in place (no two tensors of the list may then overlap); any
+ * other dst[i] is dense and overlaps no src. */
+int ddpg_clip_by_global_norm(int device, void* stream, int n, const int* dtype,
+                             const void* const* src, void* const* dst, const int64_t* count,
+                             const int64_t* cols, const int64_t* ld, float clip_norm,
+                             const float* use_norm, void* ws, size_t ws_bytes, float* norm);
+
+/* MXFP4: OCP microscaling, E2M1 elements in blocks of 32 along a row under an
+ * E8M0 scale 2^(floor(log2 max|x|) - 2), rounded to nearest even, saturating.  A
+ * block with an infinity or a NaN is NaN as a whole.  A quantised matrix is two
+ * buffers in the matrix instructions' operand order (16-byte aligned, sizes by
+ * ddpg_mx_sizes); rows and columns each up to 2^24. */
+int ddpg_mx_sizes(int64_t rows, int64_t cols, size_t* code_bytes, size_t* scale_bytes);
+int ddpg_mx_quantize(int device, void* stream, int dtype, const void* x, int64_t rows,
+                     int64_t cols, int64_t row_stride, int64_t col_stride, void* codes,
+                     void* scales);
+int ddpg_mx_dequantize(int device, void* stream, const void* codes, const void* scales,
+                       int64_t rows, int64_t cols, int dtype, void* out, int64_t row_stride);
+/* y [M, N] = act(x [M, K] . w [N, K]^T + bias [N]), w quantised.  x != NULL: x is
+ * quantised on the way, with x_codes / x_scales (sizes of [M, K]) as scratch;
+ * x == NULL: they hold x.  Sums in fp32, one rounding to dtype at the end. */
+int ddpg_mx_linear(int device, void* stream, int x_dtype, const void* x, int64_t x_row_stride,
+                   int64_t x_col_stride, void* x_codes, void* x_scales, int64_t M, int64_t K,
+                   const void* w_codes, const void* w_scales, int64_t N, int bias_dtype,
+                   const void* bias, int act, int dtype, void* y, int64_t y_row_stride);
+/* Gradients of x . w^T + bias for dy [M, N] of type dtype, with the values the
+ * quantised x [M, K] and w [N, K] stand for (straight-through: the quantisation's
+ * own derivative is taken as 1): dx [M, K] = dy . w (of type dtype), dw [N, K] =
+ * dy^T . x, db [N] = column sums (fp32), all dense.  dy enters exactly (as one,
+ * two or three bfloat16 planes), sums are fp32.  Outputs may be NULL; x is read
+ * for dw only, w for dx only. */
+size_t ddpg_mx_linear_grad_workspace(int dtype, int64_t M, int64_t N, int64_t K, int dx, int dw,
+                                     int db);
+int ddpg_mx_linear_grad(int device, void* stream, int dtype, const void* dy,
+                        int64_t dy_row_stride, int64_t dy_col_stride, int64_t M, int64_t N,
+                        int64_t K, const void* x_codes, const void* x_scales,
+                        const void* w_codes, const void* w_scales, void* dx, float* dw, float* db,
+                        void* ws, size_t ws_bytes);
 
 /* ------------------------------------------------------------- checkpoints */
 /* CRC-32C (Castagnoli) of n bytes continuing from crc (0 to start): the checksum
