@@ -1,7 +1,7 @@
 // MXFP4 operators: quantisation and its inverse, the product of two quantised
 // matrices (a layer's forward), and that product's gradient.  The format and
 // its layout: mx.h.
-#include "mx.h"
+#include "mx_gemm.h"
 
 namespace ddpg {
 
@@ -64,61 +64,6 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(MxMat q,
   }
 }
 
-// ---------------------------------------------------------------- product
-// y[m][n] = act(sum_k x[m][k] w[n][k] + b[n]).  W is the instruction's A
-// operand and X its B: a lane then holds four consecutive n of one m.
-struct MxOut {
-  void* y;
-  const void* bias;
-  long long ldo;
-  int M, N, dtype, bias_dtype, act;
-};
-
-DDPG_DEV float mx_act(float v, int act) {
-  if (act == DDPG_ACT_ELU) return elu_f(v);
-  if (act == DDPG_ACT_TANH) return tanhf(v);
-  return v;
-}
-
-DDPG_DEV void mx_store(const MxOut& o, int m, int n, const f32x4& d) {
-  if (m >= o.M) return;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    if (n + r >= o.N) return;
-    const float b = o.bias ? load_elem(o.bias, o.bias_dtype, n + r) : 0.f;
-    store_elem(o.y, o.dtype, m * o.ldo + n + r, mx_act(__fadd_rn(d[r], b), o.act));
-  }
-}
-
-// One wave: 64 n x 64 m, operands straight from memory.
-__global__ __launch_bounds__(64) void mx_linear_kernel(MxMat x, MxMat w, MxOut o) {
-  const int kt = x.kt(), l = threadIdx.x;
-  const int nn = (o.N + 63) >> 6, mg = blockIdx.x / nn, ng = blockIdx.x % nn;
-  f32x4 acc[4][4] = {};
-  for (int k = 0; k < kt; ++k) {
-    u32x4 a[4], b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = *reinterpret_cast<const u32x4*>(w.codes + mx_code_at(ng * 4 + i, kt, k) + l * 16);
-      b[i] = *reinterpret_cast<const u32x4*>(x.codes + mx_code_at(mg * 4 + i, kt, k) + l * 16);
-    }
-    const unsigned sa = *reinterpret_cast<const unsigned*>(w.scales + mx_scale_at(ng, kt, k) + l * 4);
-    const unsigned sb = *reinterpret_cast<const unsigned*>(x.scales + mx_scale_at(mg, kt, k) + l * 4);
-#define MX_ROW(i)                                        \
-  acc[i][0] = mx_mfma<i, 0>(a[i], b[0], acc[i][0], sa, sb); \
-  acc[i][1] = mx_mfma<i, 1>(a[i], b[1], acc[i][1], sa, sb); \
-  acc[i][2] = mx_mfma<i, 2>(a[i], b[2], acc[i][2], sa, sb); \
-  acc[i][3] = mx_mfma<i, 3>(a[i], b[3], acc[i][3], sa, sb);
-    MX_ROW(0) MX_ROW(1) MX_ROW(2) MX_ROW(3)
-#undef MX_ROW
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      mx_store(o, mg * 64 + j * 16 + (l & 15), ng * 64 + i * 16 + (l >> 4) * 4, acc[i][j]);
-}
-
 // ---------------------------------------------------------------- gradient
 // dX = dY W, dW = dY^T X and db = sum_m dY with the values the quantised
 // operands stand for, which bfloat16 holds exactly.  dY goes in as bfloat16
@@ -142,10 +87,11 @@ DDPG_DEV void plane_split(float x, __bf16 (&p)[P]) {
   }
 }
 
-// out[c][r] (ldt columns, rows..ldt zero) of a quantised matrix, a 64 x 128
-// tile per block through LDS.
-__global__ __launch_bounds__(256) void mx_turn_kernel(MxMat q, __bf16* __restrict__ out, int ldt) {
-  __shared__ __bf16 t[128][66];
+// A quantised matrix turned into bfloat16 fragments (mx_gemm.h): rows are its
+// columns, the depth its rows (to whole 64s, the padding 0).  A 64 x 128 tile
+// per block, through LDS.
+__global__ __launch_bounds__(256) void mx_turn_kernel(MxMat q, uint8_t* __restrict__ out) {
+  __shared__ __attribute__((aligned(16))) __bf16 t[128][72];
   const int kt = q.kt(), g64 = blockIdx.x / kt, k = blockIdx.x % kt;
   const int g = threadIdx.x >> 6, l = threadIdx.x & 63;
   const int g16 = g64 * 4 + g;
@@ -164,39 +110,53 @@ __global__ __launch_bounds__(256) void mx_turn_kernel(MxMat q, __bf16* __restric
     for (int i = 0; i < 32; ++i) t[(l >> 4) * 32 + i][g * 16 + (l & 15)] = (__bf16)v[i];
   }
   __syncthreads();
-  for (int c = g; c < 128 && k * 128 + c < q.cols; c += 4)
-    if (g64 * 64 + l < ldt) out[(size_t)(k * 128 + c) * ldt + g64 * 64 + l] = t[c][l];
+  const int steps = (q.rows + 63) / 64 * 2;
+  for (int f = g; f < 16; f += 4) {  // 8 row groups x 2 depth steps
+    const int c = (f >> 1) * 16, d = (f & 1) * 32;
+    const size_t grp = (size_t)k * 8 + (f >> 1);
+    if (k * 128 + c >= q.cols) break;
+    *reinterpret_cast<bf16x8*>(out + (grp * steps + g64 * 2 + (f & 1)) * 1024 + l * 16) =
+        *reinterpret_cast<const bf16x8*>(&t[c + (l & 15)][d + 8 * (l >> 4)]);
+  }
 }
 
-// dY's planes as they lie ([P][M][ldn], if flat) and turned ([P][N][ldm], if
-// turned), and each 64-row block's column sums, a 64 x 64 tile per block.
+// dY's planes as fragments (mx_gemm.h; a row group's planes one after the
+// other): flat, rows m and depth n (if not null); turned, rows n and depth m (if
+// not null); both depths to whole 64s, the padding 0.  And each 64-row
+// block's column sums (part, if not null).  A 64 x 64 tile per block.
 template <int DT, int P>
 __global__ __launch_bounds__(256) void mx_dy_kernel(const typename Elem<DT>::type* __restrict__ dy,
                                                     long long sr, long long sc, int M, int N,
-                                                    __bf16* __restrict__ flat, int ldn,
-                                                    __bf16* __restrict__ turned, int ldm,
+                                                    uint8_t* __restrict__ flat,
+                                                    uint8_t* __restrict__ turned,
                                                     float* __restrict__ part) {
   __shared__ float t[64][65];
-  const int nn = (N + 63) >> 6, mb = blockIdx.x / nn, m0 = mb * 64, n0 = (blockIdx.x % nn) * 64;
+  const int nn = (N + 63) >> 6, mb = blockIdx.x / nn, nb = blockIdx.x % nn;
+  const int m0 = mb * 64, n0 = nb * 64, nm = (M + 63) >> 6;
   const int w = threadIdx.x >> 6, l = threadIdx.x & 63;
-  for (int i = w; i < 64; i += 4) {
-    const float v = m0 + i < M && n0 + l < N ? (float)dy[(m0 + i) * sr + (n0 + l) * sc] : 0.f;
-    t[i][l] = v;
-    if (flat && m0 + i < M) {
-      __bf16 p[P];
-      plane_split<P>(v, p);
-#pragma unroll
-      for (int j = 0; j < P; ++j) flat[((size_t)j * M + m0 + i) * ldn + n0 + l] = p[j];
-    }
-  }
+  for (int i = w; i < 64; i += 4)
+    t[i][l] = m0 + i < M && n0 + l < N ? (float)dy[(m0 + i) * sr + (n0 + l) * sc] : 0.f;
   __syncthreads();
-  if (turned)
-    for (int i = w; i < 64 && n0 + i < N; i += 4) {
-      __bf16 p[P];
-      plane_split<P>(t[l][i], p);
+  // 4 row groups x 2 depth steps: a wave takes row group w
+  auto put = [&](uint8_t* out, int grp, int steps, int s0, auto at) {
 #pragma unroll
-      for (int j = 0; j < P; ++j) turned[((size_t)j * N + n0 + i) * ldm + m0 + l] = p[j];
+    for (int d = 0; d < 2; ++d) {
+      bf16x8 f[P];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        __bf16 p[P];
+        plane_split<P>(at(w * 16 + (l & 15), d * 32 + 8 * (l >> 4) + e), p);
+#pragma unroll
+        for (int j = 0; j < P; ++j) f[j][e] = p[j];
+      }
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+        *reinterpret_cast<bf16x8*>(out + (((size_t)grp * P + j) * steps + s0 + d) * 1024 + l * 16) =
+            f[j];
     }
+  };
+  if (flat) put(flat, mb * 4 + w, nn * 2, nb * 2, [&](int r, int c) { return t[r][c]; });
+  if (turned) put(turned, nb * 4 + w, nm * 2, mb * 2, [&](int r, int c) { return t[c][r]; });
   if (part && w == 0 && n0 + l < N) {
     float s = 0.f;
     for (int i = 0; i < 64; ++i) s += t[i][l];
@@ -211,42 +171,6 @@ __global__ __launch_bounds__(256) void mx_db_kernel(const float* __restrict__ pa
   double s = 0;
   for (int i = 0; i < np; ++i) s += part[(size_t)i * N + n];
   db[n] = (float)s;
-}
-
-// C[i][j] = sum_p sum_k A[p][i][k] B[j][k]; one wave: 64 x 64, operands straight
-// from memory.  ld: the padded contraction length of both.
-__global__ __launch_bounds__(64) void mx_plane_gemm_kernel(const __bf16* __restrict__ A,
-                                                           const __bf16* __restrict__ B, int I,
-                                                           int J, int ld, int planes, void* C,
-                                                           int dtype) {
-  const int nj = (J + 63) >> 6;
-  const int l = threadIdx.x, i0 = blockIdx.x / nj * 64, j0 = blockIdx.x % nj * 64;
-  f32x4 acc[4][4] = {};
-  for (int p = 0; p < planes; ++p)
-    for (int k = 0; k < ld; k += 32) {
-      bf16x8 a[4], b[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const size_t i = (size_t)p * I + min(i0 + t * 16 + (l & 15), I - 1);
-        const size_t j = min(j0 + t * 16 + (l & 15), J - 1);
-        a[t] = *reinterpret_cast<const bf16x8*>(A + i * ld + k + 8 * (l >> 4));
-        b[t] = *reinterpret_cast<const bf16x8*>(B + j * ld + k + 8 * (l >> 4));
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int y = 0; y < 4; ++y)
-          acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[y], a[x], acc[x][y], 0, 0, 0);
-    }
-#pragma unroll
-  for (int x = 0; x < 4; ++x)
-#pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const int i = i0 + x * 16 + (l & 15), j = j0 + y * 16 + (l >> 4) * 4;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (i < I && j + r < J) store_elem(C, dtype, (long long)i * J + j + r, acc[x][y][r]);
-    }
 }
 
 // ---------------------------------------------------------------- host
@@ -284,68 +208,94 @@ void mx_quantize_launch(hipStream_t st, int dtype, const void* x, int rows, int 
   HIP_TRY(hipGetLastError());
 }
 
-void mx_linear_launch(hipStream_t st, const MxMat& x, const MxMat& w, const MxOut& o) {
-  if (!o.M || !o.N) return;
-  hipLaunchKernelGGL(mx_linear_kernel, dim3(grid_x((long long)ceil_div(o.N, 64) * ceil_div(o.M, 64))),
-                     dim3(64), 0, st,
-                     x, w, o);
+// Which kernel a product of I x J outputs takes: the largest tile that leaves
+// most of the 256 CUs one, and with fewer tiles the kernel that splits the depth
+// over a block's waves.  fp4, us: 16384 x 8192 x 8192 665 on 256 x 256 tiles, 719
+// on 128 x 128; 1001 x 300 x 400 14.0 on 128 x 128 tiles, 6.7 split.  bf16: 8192 x 4096
+// x 4096 207 against 268, 1001 x 400 x 3 planes of 300 28.4 against 11.0.
+template <bool FP4>
+static void mx_gemm_launch(hipStream_t st, MxGemm g) {
+  MxOut& o = g.o;
+  if (!o.I || !o.J) return;
+  const int es = elem_size(o.dtype);
+  o.vec = o.ldo % 4 == 0 && ((uintptr_t)o.y & (4 * es - 1)) == 0;
+  const long long big = (long long)ceil_div(o.I, 256) * ceil_div(o.J, 256);
+  const long long mid = (long long)ceil_div(o.I, 128) * ceil_div(o.J, 128);
+  if (big >= 200) {
+    hipLaunchKernelGGL((mx_tile_kernel<FP4, 2, 4, 8, 4, 4>), dim3(grid_x(big)), dim3(512), 0, st, g);
+  } else if (mid >= 128) {
+    hipLaunchKernelGGL((mx_tile_kernel<FP4, 2, 2, 4, 4, 4>), dim3(grid_x(mid)), dim3(256), 0, st, g);
+  } else if (o.I <= 16) {
+    hipLaunchKernelGGL((mx_split_kernel<FP4, 1, 1, 8>), dim3(ceil_div(o.J, 16)), dim3(512), 0, st,
+                       g);
+  } else {
+    const long long small = (long long)ceil_div(o.I, 64) * ceil_div(o.J, 64);
+    hipLaunchKernelGGL((mx_split_kernel<FP4, 4, 4, 4>), dim3(grid_x(small)), dim3(256), 0, st, g);
+  }
   HIP_TRY(hipGetLastError());
+}
+
+static FragOp mx_op(const MxMat& q) {
+  return {q.codes, q.scales, ceil_div(q.rows, 64) * 4};
+}
+
+void mx_linear_launch(hipStream_t st, const MxMat& x, const MxMat& w, const MxOut& o) {
+  mx_gemm_launch<true>(st, MxGemm{mx_op(x), mx_op(w), x.kt(), 1, o});
 }
 
 // The gradient's workspace, in order.
 struct MxGradWs {
   size_t flat, wt, turned, xt, part, total;
-  int ldn, ldm, P;
+  int sn, sm, P;  // depth steps over N, over M
 };
 static MxGradWs mx_grad_ws(int dtype, int M, int N, int K, bool dx, bool dw, bool db) {
   MxGradWs w{};
   w.P = mx_planes(dtype);
-  w.ldn = rup(N, 64);
-  w.ldm = rup(M, 64);
+  w.sn = ceil_div(N, 64) * 2;
+  w.sm = ceil_div(M, 64) * 2;
+  auto frags = [](int rows, size_t steps) { return (size_t)ceil_div(rows, 64) * 4 * steps * 1024; };
   size_t off = 0;
   auto place = [&](size_t& at, bool need, size_t bytes) {
     at = off;
     if (need) off += (bytes + 255) / 256 * 256;
   };
-  place(w.flat, dx, (size_t)w.P * M * w.ldn * 2);
-  place(w.wt, dx, (size_t)K * w.ldn * 2);
-  place(w.turned, dw, (size_t)w.P * N * w.ldm * 2);
-  place(w.xt, dw, (size_t)K * w.ldm * 2);
+  place(w.flat, dx, frags(M, (size_t)w.P * w.sn));
+  place(w.wt, dx, frags(K, w.sn));
+  place(w.turned, dw, frags(N, (size_t)w.P * w.sm));
+  place(w.xt, dw, frags(K, w.sm));
   place(w.part, db, (size_t)ceil_div(M, 64) * N * 4);
   w.total = off;
   return w;
 }
 
-static void mx_plane_gemm(hipStream_t st, const __bf16* A, const __bf16* B, int I, int J, int ld,
-                          int planes, void* C, int dtype) {
-  if (!I || !J) return;
-  hipLaunchKernelGGL(mx_plane_gemm_kernel, dim3(grid_x((long long)ceil_div(J, 64) * ceil_div(I, 64))),
-                     dim3(64), 0, st, A, B, I, J, ld, planes, C, dtype);
+static void mx_turn(hipStream_t st, const MxMat& q, uint8_t* out) {
+  if (!q.rows || !q.cols) return;
+  hipLaunchKernelGGL(mx_turn_kernel, dim3(grid_x((long long)q.kt() * ceil_div(q.rows, 64))),
+                     dim3(256), 0, st, q, out);
   HIP_TRY(hipGetLastError());
 }
 
-static void mx_turn(hipStream_t st, const MxMat& q, __bf16* out, int ldt) {
-  if (!q.rows || !q.cols) return;
-  hipLaunchKernelGGL(mx_turn_kernel, dim3(grid_x((long long)q.kt() * ceil_div(q.rows, 64))), dim3(256), 0,
-                     st, q, out,
-                     ldt);
-  HIP_TRY(hipGetLastError());
+static void mx_plane_gemm(hipStream_t st, const uint8_t* A, const uint8_t* B, int I, int J,
+                          int steps, int planes, void* C, int dtype) {
+  const MxOut o{C, nullptr, J, I, J, dtype, 0, DDPG_ACT_NONE, 0};
+  mx_gemm_launch<false>(st, MxGemm{{A, nullptr, ceil_div(I, 64) * 4},
+                                   {B, nullptr, ceil_div(J, 64) * 4}, steps, planes, o});
 }
 
 void mx_linear_grad_launch(hipStream_t st, int dtype, const void* dy, long long sr, long long sc,
                            const MxMat& x, const MxMat& w, void* dx, float* dw, float* db,
-                           char* ws) {
+                           uint8_t* ws) {
   const int M = x.rows, N = w.rows, K = x.cols;
   const MxGradWs L = mx_grad_ws(dtype, M, N, K, dx, dw, db);
-  __bf16* flat = dx ? reinterpret_cast<__bf16*>(ws + L.flat) : nullptr;
-  __bf16* turned = dw ? reinterpret_cast<__bf16*>(ws + L.turned) : nullptr;
+  uint8_t* flat = dx ? ws + L.flat : nullptr;
+  uint8_t* turned = dw ? ws + L.turned : nullptr;
   float* part = db ? reinterpret_cast<float*>(ws + L.part) : nullptr;
-  if (M && N) {
+  if (M && N && (dx || dw || db)) {
     by_dtype(dtype, [&](auto dt) {
       hipLaunchKernelGGL((mx_dy_kernel<dt.value, mx_planes(dt.value)>),
-                         dim3(grid_x((long long)ceil_div(N, 64) * ceil_div(M, 64))), dim3(256), 0, st,
-                         static_cast<const typename Elem<dt.value>::type*>(dy), sr, sc, M, N, flat,
-                         L.ldn, turned, L.ldm, part);
+                         dim3(grid_x((long long)ceil_div(N, 64) * ceil_div(M, 64))), dim3(256), 0,
+                         st, static_cast<const typename Elem<dt.value>::type*>(dy), sr, sc, M, N,
+                         flat, turned, part);
     });
     HIP_TRY(hipGetLastError());
   }
@@ -355,14 +305,12 @@ void mx_linear_grad_launch(hipStream_t st, int dtype, const void* dy, long long 
     HIP_TRY(hipGetLastError());
   }
   if (dx) {
-    __bf16* wt = reinterpret_cast<__bf16*>(ws + L.wt);
-    mx_turn(st, w, wt, L.ldn);
-    mx_plane_gemm(st, flat, wt, M, K, L.ldn, L.P, dx, dtype);
+    mx_turn(st, w, ws + L.wt);
+    mx_plane_gemm(st, flat, ws + L.wt, M, K, L.sn, L.P, dx, dtype);
   }
   if (dw) {
-    __bf16* xt = reinterpret_cast<__bf16*>(ws + L.xt);
-    mx_turn(st, x, xt, L.ldm);
-    mx_plane_gemm(st, turned, xt, N, K, L.ldm, L.P, dw, T_FP32);
+    mx_turn(st, x, ws + L.xt);
+    mx_plane_gemm(st, turned, ws + L.xt, N, K, L.sm, L.P, dw, T_FP32);
   }
 }
 
@@ -429,7 +377,7 @@ int ddpg_mx_linear(int device, void* stream, int x_dtype, const void* x, int64_t
     if (x)
       mx_quantize_launch(st, x_dtype, x, (int)M, (int)K, x_row_stride, x_col_stride,
                          static_cast<uint8_t*>(x_codes), static_cast<uint8_t*>(x_scales));
-    const MxOut o{y, bias, (long long)y_row_stride, (int)M, (int)N, dtype, bias_dtype, act};
+    const MxOut o{y, bias, (long long)y_row_stride, (int)M, (int)N, dtype, bias_dtype, act, 0};
     mx_linear_launch(st, xq, wq, o);
   });
 }
@@ -460,7 +408,7 @@ int ddpg_mx_linear_grad(int device, void* stream, int dtype, const void* dy, int
     MxMat xm = xq, wm = wq;
     xm.cols = wm.cols = (int)K;
     mx_linear_grad_launch(static_cast<hipStream_t>(stream), dtype, dy, dy_row_stride, dy_col_stride,
-                          xm, wm, dx, dw, db, static_cast<char*>(ws));
+                          xm, wm, dx, dw, db, static_cast<uint8_t*>(ws));
   });
 }
 

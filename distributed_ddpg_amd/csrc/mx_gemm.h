@@ -1,0 +1,405 @@
+// Products of operands laid out in matrix-instruction order (gfx950):
+//   C[i][j] = sum_k I[i][k] J[j][k]
+// A fragment is 16 rows of one instruction's depth, 1 KiB, lane l's 16 bytes at
+// 16 l: 128 MXFP4 columns (mx.h) or 32 bfloat16 columns (lane l: row l % 16,
+// columns 8 (l / 16) ..).  An operand is [row groups of 16][depth steps][1 KiB],
+// row groups padded to whole fours.  Both kinds take as many cycles per
+// fragment pair (v_mfma_scale_f32_16x16x128_f8f6f4 on fp4, 4 times the rate of
+// v_mfma_f32_16x16x32_bf16), so one kernel serves both.
+//
+// J is the instruction's first operand: lane l holds C[i = l % 16] of four
+// consecutive j = 4 (l / 16) .. +3, which are adjacent in memory.
+#pragma once
+#include "gemm_h256.h"
+#include "mx.h"
+
+namespace ddpg {
+
+// What becomes of C: y = act(C + bias), rounded once to dtype.
+struct MxOut {
+  void* y;
+  const void* bias;
+  long long ldo;
+  int I, J, dtype, bias_dtype, act;
+  int vec;  // four adjacent outputs are one aligned store
+};
+
+struct FragOp {
+  const uint8_t* p;       // fragments
+  const uint8_t* scales;  // mx.h's scales, or null
+  int groups;             // 16-row groups held (a multiple of 4)
+};
+
+struct MxGemm {
+  FragOp I, J;
+  int kt;      // depth steps of J
+  int planes;  // I holds `planes` times kt steps a row group; J's repeat
+  MxOut o;
+};
+
+DDPG_DEV float mx_act(float v, int act) {
+  if (act == DDPG_ACT_ELU) return elu_f(v);
+  if (act == DDPG_ACT_TANH) return tanhf(v);
+  return v;
+}
+
+// C[i][j .. j+3] of a lane to the output; b: the four biases
+DDPG_DEV void mx_store(const MxOut& o, int i, int j, const f32x4& d, const float* b) {
+  if (i >= o.I || j >= o.J) return;
+  float v[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = mx_act(__fadd_rn(d[r], b[r]), o.act);
+  const long long at = i * o.ldo + j;
+  if (o.vec && j + 4 <= o.J) {
+    if (o.dtype == T_FP32) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(o.y) + at) = f32x4{v[0], v[1], v[2], v[3]};
+    } else if (o.dtype == T_BF16) {
+      const bf16x4 h = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+      *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(o.y) + at) = h;
+    } else {
+      typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+      const f16x4 h = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+      *reinterpret_cast<f16x4*>(static_cast<_Float16*>(o.y) + at) = h;
+    }
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (j + r < o.J) store_elem(o.y, o.dtype, at + r, v[r]);
+}
+
+DDPG_DEV void mx_bias(const MxOut& o, int j, float* b) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    b[r] = o.bias && j + r < o.J ? load_elem(o.bias, o.bias_dtype, j + r) : 0.f;
+}
+
+// acc[j + r][i] += J fragment x I fragment, with scale bytes BJ of sj, BI of si
+template <bool FP4, int BJ, int BI>
+DDPG_DEV f32x4 frag_mfma(const u32x4& j, const u32x4& i, f32x4 acc, unsigned sj, unsigned si) {
+  if constexpr (FP4)
+    return mx_mfma<BJ, BI>(j, i, acc, sj, si);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, j),
+                                                   __builtin_bit_cast(bf16x8, i), acc, 0, 0, 0);
+}
+
+// Tile of a block.  The grid is one-dimensional: every XCD (workgroups are
+// dealt to the 8 in turn) takes a contiguous run of the order, which walks
+// eight rows of tiles down before it steps across, so that the tiles an XCD
+// works on at once share their operands in its L2.
+DDPG_DEV void tile_of(int ni, int nj, int& ti, int& tj) {
+  const int n = ni * nj, lin = blockIdx.x;
+  const int x = lin & 7, q = n >> 3, r = n & 7;
+  const int t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (lin >> 3);
+  const int band = t / (8 * nj), in = t - band * 8 * nj;
+  const int rows = min(8, ni - band * 8);
+  ti = band * 8 + in % rows;
+  tj = in / rows;
+}
+
+// ---------------------------------------------------------------- LDS tiles
+template <int OFF>
+DDPG_DEV u32x4 lds_b128(unsigned a) {
+  u32x4 r;
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(a), "n"(OFF));
+  return r;
+}
+template <int OFF>
+DDPG_DEV unsigned lds_b32(unsigned a) {
+  unsigned r;
+  asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(r) : "v"(a), "n"(OFF));
+  return r;
+}
+
+// 16 (4) bytes a lane from memory to LDS, lane after lane.  A plain function: in
+// a kernel template the builtin keeps hipcc from emitting the launch stub.
+DDPG_DEV void lds_load16(const uint8_t* p, lds_char* to) {
+  __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)p, (lds_void*)to, 16, 0,
+                                   0);
+}
+DDPG_DEV void lds_load4(const uint8_t* p, lds_char* to) {
+  __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)p, (lds_void*)to, 4, 0,
+                                   0);
+}
+
+// WI x WJ waves of TI x TJ fragments each, a ring of NS depth steps in LDS.
+template <bool FP4, int WI, int WJ, int TI, int TJ, int NS>
+struct RingCfg {
+  static constexpr int NW = WI * WJ, NT = 64 * NW;
+  static constexpr int GI = WI * TI, GJ = WJ * TJ;  // fragments of a step
+  static constexpr int PW = (GI + GJ) / NW;         // of them loaded by a wave
+  static constexpr int SP = FP4 ? (GI + GJ) / 4 : 0;  // 256-byte scale pieces
+  static constexpr int SW = SP / NW;
+  static constexpr int SLOT = (GI + GJ) * 1024 + SP * 256;
+  static constexpr int LDS = NS * SLOT;
+  static_assert(PW * NW == GI + GJ && SW * NW == SP && TI % 4 == 0 && TJ % 4 == 0, "whole pieces");
+  static_assert(LDS <= 160 * 1024, "LDS");
+  static_assert((GI + GJ) * 1024 + SP * 256 < 65536, "LDS offsets are immediates");
+};
+
+// Depth steps s .. s + NS - 1 are in LDS or on their way (global_load_lds, 16
+// bytes a lane) while the wave multiplies step s from registers.  Per step: wait
+// for the own loads of s + 1; one barrier (so s + 1 is whole and nobody reads s
+// any more); then the products, with the LDS reads of s + 1 and the loads of
+// s + NS between them; wait for the reads.  An I fragment's registers are
+// refilled after its last use, the J fragments, the last I fragment and the
+// scales have two sets.  The LDS reads are inline asm because the compiler would
+// drain the loads in flight before reads of its own; the wait that ends the step
+// is tied to their registers, so none is touched while a read is under way.
+template <bool FP4, int WI, int WJ, int TI, int TJ, int NS>
+__global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemm g) {
+  using C = RingCfg<FP4, WI, WJ, TI, TJ, NS>;
+  __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wi = wave / WJ, wj = wave % WJ;
+  const int ni = (g.o.I + C::GI * 16 - 1) / (C::GI * 16);
+  const int nj = (g.o.J + C::GJ * 16 - 1) / (C::GJ * 16);
+  int ti, tj;
+  tile_of(ni, nj, ti, tj);
+  const int nk = g.kt * g.planes;
+
+  // this wave's pieces of a step: source of the next step to load, LDS place.
+  // Row groups past the operand's last are read from the last one's place
+  // (their results are not stored).
+  const uint8_t* src[C::PW];
+  const uint8_t* ssrc[C::SW + 1];
+  bool isj[C::PW];
+#pragma unroll
+  for (int p = 0; p < C::PW; ++p) {
+    const int f = wave * C::PW + p;
+    isj[p] = f >= C::GI;
+    const int grp = isj[p] ? min(tj * C::GJ + f - C::GI, g.J.groups - 1)
+                           : min(ti * C::GI + f, g.I.groups - 1);
+    src[p] = (isj[p] ? g.J.p + (size_t)grp * g.kt * 1024 : g.I.p + (size_t)grp * nk * 1024) +
+             lane * 16;
+  }
+#pragma unroll
+  for (int p = 0; p < C::SW; ++p) {
+    const int f = wave * C::SW + p;
+    const bool j = f >= C::GI / 4;
+    const int grp = j ? min(tj * (C::GJ / 4) + f - C::GI / 4, g.J.groups / 4 - 1)
+                      : min(ti * (C::GI / 4) + f, g.I.groups / 4 - 1);
+    ssrc[p] = (j ? g.J.scales : g.I.scales) + (size_t)grp * g.kt * 256 + lane * 4;
+  }
+  int jk = 0;  // J's depth step of the next load (I's planes go on, J's repeat)
+  lds_char* const base = (lds_char*)smem;
+  auto load_piece = [&](int slot, auto p_c) {
+    constexpr int p = decltype(p_c)::value;
+    if constexpr (p < C::PW) {
+      lds_load16(src[p], base + slot * C::SLOT + (wave * C::PW + p) * 1024);
+      src[p] += 1024;
+      if (!FP4 && isj[p] && jk + 1 == g.kt) src[p] -= (size_t)g.kt * 1024;
+    } else {
+      constexpr int q = p - C::PW;
+      lds_load4(ssrc[q],
+                base + slot * C::SLOT + (C::GI + C::GJ) * 1024 + (wave * C::SW + q) * 256);
+      ssrc[q] += 256;
+    }
+    if constexpr (p == C::PW + C::SW - 1) jk = jk + 1 == g.kt ? 0 : jk + 1;
+  };
+  constexpr int G = C::PW + C::SW;
+  constexpr int NM = TI * TJ;
+  static_assert(NM >= TJ + 1 + G && NM >= 2 * TJ, "gaps for the loads and the reads");
+
+  f32x4 acc[TI][TJ];
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (nk > 0) {
+    u32x4 fi[TI], fl[2], fj[2][TJ];  // fi[TI - 1] is fl
+    unsigned si[2][TI / 4] = {}, sj[2][TJ / 4] = {};
+    const unsigned lb = (unsigned)(uintptr_t)base;
+    const unsigned bi = lb + lane * 16 + wi * TI * 1024;
+    const unsigned bj = lb + lane * 16 + (C::GI + wj * TJ) * 1024;
+    const unsigned bs = lb + lane * 4 + (C::GI + C::GJ) * 1024;
+    const unsigned bsi = bs + wi * (TI / 4) * 256;
+    const unsigned bsj = bs + (C::GI / 4 + wj * (TJ / 4)) * 256;
+    auto read_i = [&](auto set_c, auto i_c, unsigned so) {
+      constexpr int set = decltype(set_c)::value, i = decltype(i_c)::value;
+      (i == TI - 1 ? fl[set] : fi[i]) = lds_b128<i * 1024>(bi + so);
+    };
+    auto read_j = [&](auto set_c, auto j_c, unsigned so) {
+      constexpr int set = decltype(set_c)::value, j = decltype(j_c)::value;
+      fj[set][j] = lds_b128<j * 1024>(bj + so);
+    };
+    auto read_s = [&](auto set_c, unsigned so) {
+      constexpr int set = decltype(set_c)::value;
+      if constexpr (FP4) {
+        static_for<TI / 4>([&](auto c) { si[set][decltype(c)::value] = lds_b32<decltype(c)::value * 256>(bsi + so); });
+        static_for<TJ / 4>([&](auto c) { sj[set][decltype(c)::value] = lds_b32<decltype(c)::value * 256>(bsj + so); });
+      }
+    };
+    // the reads issued so far have landed in set `set`
+    auto landed = [&](auto set_c) {
+      constexpr int set = decltype(set_c)::value;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < TI - 1; ++i) asm volatile("" : "+v"(fi[i]));
+      asm volatile("" : "+v"(fl[set]));
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) asm volatile("" : "+v"(fj[set][j]));
+      if constexpr (FP4) {
+#pragma unroll
+        for (int i = 0; i < TI / 4; ++i) asm volatile("" : "+v"(si[set][i]));
+#pragma unroll
+        for (int j = 0; j < TJ / 4; ++j) asm volatile("" : "+v"(sj[set][j]));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // one step from register set SET.  RT: near the end, where step s + 1 or
+    // s + NS may not exist
+    auto step = [&](int s, auto set_c, auto rt_c) {
+      constexpr int SET = decltype(set_c)::value;
+      constexpr bool RT = decltype(rt_c)::value;
+      using Other = std::integral_constant<int, SET ^ 1>;
+      const bool next = !RT || s + 1 < nk, stage = !RT || s + NS < nk;
+      if (RT && s + NS > nk)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * G) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      const unsigned so = (unsigned)((s + 1) % NS) * C::SLOT;
+      const int slot = s % NS;
+      static_for<NM>([&](auto q_c) {
+        constexpr int q = decltype(q_c)::value, i = q / TJ, j = q % TJ;
+        acc[i][j] = frag_mfma<FP4, j % 4, i % 4>(fj[SET][j], i == TI - 1 ? fl[SET] : fi[i], acc[i][j],
+                                                 sj[SET][j / 4], si[SET][i / 4]);
+        if (next) {
+          if constexpr (q < TJ) read_j(Other{}, q_c, so);
+          if constexpr (q == TJ - 1) read_i(Other{}, std::integral_constant<int, TI - 1>{}, so);
+          if constexpr (q == TJ) read_s(Other{}, so);
+          if constexpr (i >= 1 && j == 0) read_i(Other{}, std::integral_constant<int, i - 1>{}, so);
+        }
+        constexpr int gap = (NM - TJ - 1) / G;
+        if constexpr (q > TJ && (q - TJ - 1) % gap == 0 && (q - TJ - 1) / gap < G)
+          if (stage) load_piece(slot, std::integral_constant<int, (q - TJ - 1) / gap>{});
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      landed(Other{});
+    };
+    // the first NS steps on their way, step 0 landed, its fragments read
+    for (int s = 0; s < NS && s < nk; ++s)
+      static_for<G>([&](auto p_c) { load_piece(s, p_c); });
+    if (nk >= NS)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * G) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    using S0 = std::integral_constant<int, 0>;
+    using S1 = std::integral_constant<int, 1>;
+    static_for<TI>([&](auto c) { read_i(S0{}, c, 0u); });
+    static_for<TJ>([&](auto c) { read_j(S0{}, c, 0u); });
+    read_s(S0{}, 0u);
+    landed(S0{});
+    int s = 0;
+    for (; s + 1 + NS < nk; s += 2) {
+      step(s, S0{}, std::false_type{});
+      step(s + 1, S1{}, std::false_type{});
+    }
+    for (; s < nk; s += 2) {
+      step(s, S0{}, std::true_type{});
+      if (s + 1 < nk) step(s + 1, S1{}, std::true_type{});
+    }
+  }
+  const int i0 = (ti * C::GI + wi * TI) * 16 + (lane & 15);
+  const int j0 = (tj * C::GJ + wj * TJ) * 16 + (lane >> 4) * 4;
+#pragma unroll
+  for (int j = 0; j < TJ; ++j) {
+    float b[4];
+    mx_bias(g.o, j0 + j * 16, b);
+#pragma unroll
+    for (int i = 0; i < TI; ++i) mx_store(g.o, i0 + i * 16, j0 + j * 16, acc[i][j], b);
+  }
+}
+
+// ---------------------------------------------------------------- few tiles
+// One block: TI x TJ fragments of C, its NW waves taking every NW-th depth step
+// with operands straight from memory, two steps ahead; the waves' sums are
+// joined in LDS in wave order.
+template <bool FP4, int TI, int TJ, int NW>
+__global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemm g) {
+  __shared__ f32x4 part[NW][TI * TJ][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ni = (g.o.I + TI * 16 - 1) / (TI * 16), nj = (g.o.J + TJ * 16 - 1) / (TJ * 16);
+  int ti, tj;
+  tile_of(ni, nj, ti, tj);
+  const int nk = g.kt * g.planes;
+  f32x4 acc[TI][TJ];
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const uint8_t *pi[TI], *pj[TJ];
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+    pi[i] = g.I.p + (size_t)min(ti * TI + i, g.I.groups - 1) * nk * 1024 + lane * 16;
+#pragma unroll
+  for (int j = 0; j < TJ; ++j)
+    pj[j] = g.J.p + (size_t)min(tj * TJ + j, g.J.groups - 1) * g.kt * 1024 + lane * 16;
+  // the scale dwords of the 64-row groups the fragments lie in (TI, TJ: 1 or 4)
+  const int gi = ti * TI, gj = tj * TJ;
+  const uint8_t* qi = FP4 ? g.I.scales + (size_t)min(gi >> 2, g.I.groups / 4 - 1) * g.kt * 256 + lane * 4 : nullptr;
+  const uint8_t* qj = FP4 ? g.J.scales + (size_t)min(gj >> 2, g.J.groups / 4 - 1) * g.kt * 256 + lane * 4 : nullptr;
+  struct Step {
+    u32x4 i[TI], j[TJ];
+    unsigned si, sj;
+  };
+  auto load = [&](int s, Step& f) {
+    const int k = FP4 ? s : s % g.kt;
+#pragma unroll
+    for (int i = 0; i < TI; ++i) f.i[i] = *reinterpret_cast<const u32x4*>(pi[i] + (size_t)s * 1024);
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) f.j[j] = *reinterpret_cast<const u32x4*>(pj[j] + (size_t)k * 1024);
+    f.si = f.sj = 0;
+    if constexpr (FP4) {
+      f.si = *reinterpret_cast<const unsigned*>(qi + (size_t)k * 256);
+      f.sj = *reinterpret_cast<const unsigned*>(qj + (size_t)k * 256);
+      if (TI == 1) f.si >>= 8 * (gi & 3);
+      if (TJ == 1) f.sj >>= 8 * (gj & 3);
+    }
+  };
+  auto mul = [&](const Step& f) {
+    static_for<TI * TJ>([&](auto q_c) {
+      constexpr int i = decltype(q_c)::value / TJ, j = decltype(q_c)::value % TJ;
+      acc[i][j] = frag_mfma<FP4, j, i>(f.j[j], f.i[i], acc[i][j], f.sj, f.si);
+    });
+  };
+  {
+    Step a, b;
+    int s = wave;
+    if (s < nk) load(s, a);
+    if (s + NW < nk) load(s + NW, b);
+    for (; s < nk; s += 2 * NW) {
+      mul(a);
+      if (s + 2 * NW < nk) load(s + 2 * NW, a);
+      if (s + NW < nk) {
+        mul(b);
+        if (s + 3 * NW < nk) load(s + 3 * NW, b);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) part[wave][i * TJ + j][lane] = acc[i][j];
+  __syncthreads();
+  for (int f = wave; f < TI * TJ; f += NW) {
+    f32x4 s = part[0][f][lane];
+    for (int w = 1; w < NW; ++w) s += part[w][f][lane];
+    const int i = f / TJ, j = f % TJ;
+    const int jj = (tj * TJ + j) * 16 + (lane >> 4) * 4;
+    float b[4];
+    mx_bias(g.o, jj, b);
+    mx_store(g.o, (ti * TI + i) * 16 + (lane & 15), jj, s, b);
+  }
+}
+
+}  // namespace ddpg
