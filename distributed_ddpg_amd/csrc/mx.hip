@@ -218,7 +218,7 @@ static void mx_gemm_launch(hipStream_t st, MxGemm g) {
   MxOut& o = g.o;
   if (!o.I || !o.J) return;
   const int es = elem_size(o.dtype);
-  o.vec = o.ldo % 4 == 0 && ((uintptr_t)o.y & (4 * es - 1)) == 0;
+  o.vec = o.ldo * es % 16 == 0 && aligned16(o.y);
   const long long big = (long long)ceil_div(o.I, 256) * ceil_div(o.J, 256);
   const long long mid = (long long)ceil_div(o.I, 128) * ceil_div(o.J, 128);
   if (big >= 200) {

@@ -21,7 +21,7 @@ struct MxOut {
   const void* bias;
   long long ldo;
   int I, J, dtype, bias_dtype, act;
-  int vec;  // four adjacent outputs are one aligned store
+  int vec;  // rows begin on 16-byte boundaries
 };
 
 struct FragOp {
@@ -72,6 +72,54 @@ DDPG_DEV void mx_bias(const MxOut& o, int j, float* b) {
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     b[r] = o.bias && j + r < o.J ? load_elem(o.bias, o.bias_dtype, j + r) : 0.f;
+}
+
+// A wave's TI x TJ fragments to the output by whole rows: 16 rows at a time go
+// through a strip of LDS of its own (two in turn), from where 8 (bf16, fp16) or
+// 16 (fp32) lanes write a row's 64 outputs as 16-byte stores.  Straight from the
+// registers a store covers 32 bytes of a row, and the write-out cost 28 us a
+// 256 x 256 tile.
+template <int DT, int TI, int TJ>
+DDPG_DEV void mx_store_tile(const MxOut& o, lds_char* strip, int i0, int j0,
+                            const f32x4 (&acc)[TI][TJ], const float (&bias)[TJ][4]) {
+  typedef typename Elem<DT>::type T;
+  constexpr int ROW = TJ * 16 * sizeof(T) + 16;  // padded: rows start 4 banks apart
+  constexpr int V = 16 / sizeof(T), PER = TJ * 16 / V;  // 16-byte units of a row
+  typedef T tx4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) tx4 lds_tx4;
+  typedef __attribute__((address_space(3))) u32x4 lds_u4;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < TI; ++i) {
+    lds_char* const s = strip + (i & 1) * 16 * ROW;
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      tx4 v;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = (T)mx_act(__fadd_rn(acc[i][j][r], bias[j][r]), o.act);
+      *(lds_tx4*)(s + (lane & 15) * ROW + (j * 16 + (lane >> 4) * 4) * (int)sizeof(T)) = v;
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int u = lane; u < 16 * PER; u += 64) {
+      const int r = u / PER, c = u % PER * V;
+      const u32x4 w = *(lds_u4*)(s + r * ROW + c * (int)sizeof(T));
+      const int row = i0 + i * 16 + r, col = j0 + c;
+      if (row < o.I && col < o.J) {
+        T* p = static_cast<T*>(o.y) + row * o.ldo + col;
+        if (o.vec && col + V <= o.J) {
+          *reinterpret_cast<u32x4*>(p) = w;
+        } else {
+          T e[V];
+          __builtin_memcpy(e, &w, 16);
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            if (col + k < o.J) p[k] = e[k];
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
 }
 
 // acc[j + r][i] += J fragment x I fragment, with scale bytes BJ of sj, BI of si
@@ -308,15 +356,16 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemm g) {
       if (s + 1 < nk) step(s + 1, S1{}, std::true_type{});
     }
   }
-  const int i0 = (ti * C::GI + wi * TI) * 16 + (lane & 15);
-  const int j0 = (tj * C::GJ + wj * TJ) * 16 + (lane >> 4) * 4;
+  __syncthreads();  // the ring is done with: it carries the results out
+  float bias[TJ][4];
 #pragma unroll
-  for (int j = 0; j < TJ; ++j) {
-    float b[4];
-    mx_bias(g.o, j0 + j * 16, b);
-#pragma unroll
-    for (int i = 0; i < TI; ++i) mx_store(g.o, i0 + i * 16, j0 + j * 16, acc[i][j], b);
-  }
+  for (int j = 0; j < TJ; ++j)
+    mx_bias(g.o, (tj * C::GJ + wj * TJ + j) * 16 + (lane >> 4) * 4, bias[j]);
+  by_dtype(g.o.dtype, [&](auto dt) {
+    mx_store_tile<decltype(dt)::value, TI, TJ>(g.o, base + wave * (C::LDS / C::NW / 1024 * 1024),
+                                               (ti * C::GI + wi * TI) * 16,
+                                               (tj * C::GJ + wj * TJ) * 16, acc, bias);
+  });
 }
 
 // ---------------------------------------------------------------- few tiles
