@@ -6,61 +6,85 @@
 namespace ddpg {
 
 // ---------------------------------------------------------------- quantise
-// A wave makes 64 rows x 128 columns: lane l takes row l % 16 and 32-block
-// l / 16 of each 16-row group in turn and keeps the four scale bytes of its
-// dword.  Its 32 values are 16-byte loads when the columns are adjacent.
-template <int DT>
+// A block makes one tile of 64 rows x 128 columns, a thread one 32-block of it.
+// ROWS: a wave takes 16 rows and its lanes read along them (16-byte loads where
+// a block's columns are adjacent).  Otherwise a wave takes 32 columns and its
+// lanes 64 rows, so that a load is contiguous where rows are (a matrix in
+// checkpoint order seen turned).  Loads past the matrix are from its last
+// element and count as 0.
+template <int DT, bool ROWS>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(
     const typename Elem<DT>::type* __restrict__ x, int rows, int cols, long long sr, long long sc,
     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const int kt = (cols + 127) >> 7, l = threadIdx.x & 63;
-  const long long tile = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int g64 = (int)(tile / kt), k = (int)(tile % kt);
-  if (g64 * 64 >= rows) return;
-  const int c0 = k * 128 + (l >> 4) * 32;
-  unsigned packed = 0;
-  for (int g = 0; g < 4; ++g) {
-    const int r = g64 * 64 + g * 16 + (l & 15);
-    if (g64 * 64 + g * 16 >= rows) break;
+  __shared__ __attribute__((aligned(4))) uint8_t sb[256];
+  const int kt = (cols + 127) >> 7, l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int g64 = blockIdx.x / kt, k = blockIdx.x % kt;
+  const int r = ROWS ? w * 16 + (l & 15) : l, kb = ROWS ? l >> 4 : w;
+  const int row = g64 * 64 + r, c0 = k * 128 + kb * 32;
+  unsigned s = 0;
+  if (g64 * 64 + (r & ~15) < rows) {
     float v[32];
-    if (r < rows && c0 + 32 <= cols && sc == 1) {
+    const typename Elem<DT>::type* p = x + min(row, rows - 1) * sr;
+    if (ROWS && c0 + 32 <= cols) {
       constexpr int V = Elem<DT>::V;
-      const typename Elem<DT>::type* p = x + r * sr + c0;
 #pragma unroll
       for (int i = 0; i < 32; i += V)
-        Elem<DT>::widen(*reinterpret_cast<const U16B*>(p + i), v + i);
+        Elem<DT>::widen(*reinterpret_cast<const U16B*>(p + c0 + i), v + i);
     } else {
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        v[i] = r < rows && c0 + i < cols ? (float)x[r * sr + (c0 + i) * sc] : 0.f;
+      for (int i = 0; i < 32; ++i) v[i] = (float)p[min(c0 + i, cols - 1) * sc];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = c0 + i < cols ? v[i] : 0.f;
     }
-    unsigned s;
     const u32x4 q = mx_quantize_block(v, s);
-    packed |= s << (8 * g);
-    *reinterpret_cast<u32x4*>(codes + mx_code_at(g64 * 4 + g, kt, k) + l * 16) = q;
+    *reinterpret_cast<u32x4*>(codes + mx_code_at(g64 * 4 + (r >> 4), kt, k) +
+                              (kb * 16 + (r & 15)) * 16) = q;
   }
-  *reinterpret_cast<unsigned*>(scales + mx_scale_at(g64, kt, k) + l * 4) = packed;
+  sb[(kb * 16 + (r & 15)) * 4 + (r >> 4)] = (uint8_t)s;
+  __syncthreads();
+  if (w == 0)
+    reinterpret_cast<unsigned*>(scales + mx_scale_at(g64, kt, k))[l] =
+        reinterpret_cast<const unsigned*>(sb)[l];
 }
 
+// A wave takes 16 rows x 128 columns: the codes go through LDS, so that its lanes
+// write along the rows, 16 bytes each.
 template <int DT>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(MxMat q,
                                                             typename Elem<DT>::type* out,
                                                             long long ldo) {
-  const int kt = q.kt(), l = threadIdx.x & 63;
-  const long long tile = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int g16 = (int)(tile / kt), k = (int)(tile % kt);
-  const int r = g16 * 16 + (l & 15), c0 = k * 128 + (l >> 4) * 32;
-  if (r >= q.rows || c0 >= q.cols) return;
-  const u32x4 w = *reinterpret_cast<const u32x4*>(q.codes + mx_code_at(g16, kt, k) + l * 16);
-  const unsigned s = q.scales[mx_scale_at(g16 >> 2, kt, k) + l * 4 + (g16 & 3)];
-  typename Elem<DT>::type* p = out + r * ldo + c0;
+  typedef typename Elem<DT>::type T;
+  constexpr int V = Elem<DT>::V, PER = 128 / V;  // 16-byte units of a row
+  __shared__ __attribute__((aligned(16))) uint8_t sq[4][1024];
+  __shared__ uint8_t ss[4][64];
+  const int kt = q.kt(), l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int g16 = blockIdx.x / kt * 4 + w, k = blockIdx.x % kt;
+  if (g16 * 16 < q.rows) {
+    *reinterpret_cast<u32x4*>(&sq[w][l * 16]) =
+        *reinterpret_cast<const u32x4*>(q.codes + mx_code_at(g16, kt, k) + l * 16);
+    ss[w][l] = q.scales[mx_scale_at(g16 >> 2, kt, k) + l * 4 + (g16 & 3)];
+  }
+  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int u = l; u < 16 * PER; u += 64) {
+    const int r = u / PER, c = u % PER * V;  // V columns of row r
+    const int row = g16 * 16 + r, col = k * 128 + c;
+    if (row >= q.rows || col >= q.cols) continue;
+    const int at = (c >> 5) * 16 + r;  // the lane that holds the block
     float v[8];
-    mx_values(w[i], s, v);
+    if (V == 4) {
+      mx_values(*reinterpret_cast<const uint16_t*>(&sq[w][at * 16 + (c & 31) / 2]), ss[w][at], v);
+    } else {
+      mx_values(*reinterpret_cast<const unsigned*>(&sq[w][at * 16 + (c & 31) / 2]), ss[w][at], v);
+    }
+    T* p = out + row * ldo + col;
+    if (col + V <= q.cols) {
+      *reinterpret_cast<U16B*>(p) = Elem<DT>::pack(v);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c0 + 8 * i + j < q.cols) p[8 * i + j] = (typename Elem<DT>::type)v[j];
+      for (int i = 0; i < V; ++i)
+        if (col + i < q.cols) p[i] = (T)v[i];
+    }
   }
 }
 
@@ -87,12 +111,24 @@ DDPG_DEV void plane_split(float x, __bf16 (&p)[P]) {
   }
 }
 
+// What the two products need first, one launch: blocks of three kinds, each
+// with one tile.
+struct MxPrep {
+  const void* dy;
+  long long sr, sc;
+  int M, N;
+  uint8_t *flat, *turned;  // dY's planes for dX, for dW (or null)
+  float* part;             // column sums of 64-row blocks (or null)
+  MxMat w, x;
+  uint8_t *wt, *xt;
+  int dy_blocks, w_blocks;
+};
+
 // A quantised matrix turned into bfloat16 fragments (mx_gemm.h): rows are its
-// columns, the depth its rows (to whole 64s, the padding 0).  A 64 x 128 tile
-// per block, through LDS.
-__global__ __launch_bounds__(256) void mx_turn_kernel(MxMat q, uint8_t* __restrict__ out) {
-  __shared__ __attribute__((aligned(16))) __bf16 t[128][72];
-  const int kt = q.kt(), g64 = blockIdx.x / kt, k = blockIdx.x % kt;
+// columns, the depth its rows (to whole 64s, the padding 0).  64 x 128 tile b,
+// through LDS.
+DDPG_DEV void mx_turn(const MxMat& q, uint8_t* __restrict__ out, int b, __bf16 (&t)[128][72]) {
+  const int kt = q.kt(), g64 = b / kt, k = b % kt;
   const int g = threadIdx.x >> 6, l = threadIdx.x & 63;
   const int g16 = g64 * 4 + g;
   {
@@ -120,22 +156,24 @@ __global__ __launch_bounds__(256) void mx_turn_kernel(MxMat q, uint8_t* __restri
   }
 }
 
-// dY's planes as fragments (mx_gemm.h; a row group's planes one after the
-// other): flat, rows m and depth n (if not null); turned, rows n and depth m (if
-// not null); both depths to whole 64s, the padding 0.  And each 64-row
-// block's column sums (part, if not null).  A 64 x 64 tile per block.
+// A 64 x 64 tile of dY as fragments of its planes (a row group's planes one after
+// the other): flat, rows m and depth n; turned, rows n and depth m; both depths
+// to whole 64s, the padding 0.  And the tile's column sums.
 template <int DT, int P>
-__global__ __launch_bounds__(256) void mx_dy_kernel(const typename Elem<DT>::type* __restrict__ dy,
-                                                    long long sr, long long sc, int M, int N,
-                                                    uint8_t* __restrict__ flat,
-                                                    uint8_t* __restrict__ turned,
-                                                    float* __restrict__ part) {
-  __shared__ float t[64][65];
-  const int nn = (N + 63) >> 6, mb = blockIdx.x / nn, nb = blockIdx.x % nn;
+DDPG_DEV void mx_dy(const MxPrep& a, int b, float (&t)[64][65]) {
+  const typename Elem<DT>::type* dy = static_cast<const typename Elem<DT>::type*>(a.dy);
+  const int M = a.M, N = a.N, nn = (N + 63) >> 6, mb = b / nn, nb = b % nn;
   const int m0 = mb * 64, n0 = nb * 64, nm = (M + 63) >> 6;
   const int w = threadIdx.x >> 6, l = threadIdx.x & 63;
-  for (int i = w; i < 64; i += 4)
-    t[i][l] = m0 + i < M && n0 + l < N ? (float)dy[(m0 + i) * sr + (n0 + l) * sc] : 0.f;
+  {
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      v[i] = (float)dy[min(m0 + w + 4 * i, M - 1) * a.sr + min(n0 + l, N - 1) * a.sc];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      t[w + 4 * i][l] = m0 + w + 4 * i < M && n0 + l < N ? v[i] : 0.f;
+  }
   __syncthreads();
   // 4 row groups x 2 depth steps: a wave takes row group w
   auto put = [&](uint8_t* out, int grp, int steps, int s0, auto at) {
@@ -155,22 +193,29 @@ __global__ __launch_bounds__(256) void mx_dy_kernel(const typename Elem<DT>::typ
             f[j];
     }
   };
-  if (flat) put(flat, mb * 4 + w, nn * 2, nb * 2, [&](int r, int c) { return t[r][c]; });
-  if (turned) put(turned, nb * 4 + w, nm * 2, mb * 2, [&](int r, int c) { return t[c][r]; });
-  if (part && w == 0 && n0 + l < N) {
+  if (a.flat) put(a.flat, mb * 4 + w, nn * 2, nb * 2, [&](int r, int c) { return t[r][c]; });
+  if (a.turned) put(a.turned, nb * 4 + w, nm * 2, mb * 2, [&](int r, int c) { return t[c][r]; });
+  if (a.part && w == 0 && n0 + l < N) {
     float s = 0.f;
+#pragma unroll
     for (int i = 0; i < 64; ++i) s += t[i][l];
-    part[(size_t)mb * N + n0 + l] = s;
+    a.part[(size_t)mb * N + n0 + l] = s;
   }
 }
 
-__global__ __launch_bounds__(256) void mx_db_kernel(const float* __restrict__ part, int np, int N,
-                                                    float* __restrict__ db) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
-  double s = 0;
-  for (int i = 0; i < np; ++i) s += part[(size_t)i * N + n];
-  db[n] = (float)s;
+template <int DT>
+__global__ __launch_bounds__(256) void mx_prep_kernel(MxPrep a) {
+  __shared__ __attribute__((aligned(16))) union {
+    __bf16 turn[128][72];
+    float dy[64][65];
+  } t;
+  const int b = blockIdx.x;
+  if (b < a.dy_blocks)
+    mx_dy<DT, mx_planes(DT)>(a, b, t.dy);
+  else if (b < a.dy_blocks + a.w_blocks)
+    mx_turn(a.w, a.wt, b - a.dy_blocks, t.turn);
+  else
+    mx_turn(a.x, a.xt, b - a.dy_blocks - a.w_blocks, t.turn);
 }
 
 // ---------------------------------------------------------------- host
@@ -199,40 +244,54 @@ static unsigned grid_x(long long blocks) {
 void mx_quantize_launch(hipStream_t st, int dtype, const void* x, int rows, int cols, long long sr,
                         long long sc, uint8_t* codes, uint8_t* scales) {
   if (!rows || !cols) return;
-  const long long tiles = (long long)ceil_div(rows, 64) * ceil_div(cols, 128);
+  const unsigned tiles = grid_x((long long)ceil_div(rows, 64) * ceil_div(cols, 128));
   by_dtype(dtype, [&](auto dt) {
-    hipLaunchKernelGGL(mx_quantize_kernel<dt.value>, dim3(grid_x((tiles + 3) / 4)), dim3(256), 0, st,
-                       static_cast<const typename Elem<dt.value>::type*>(x), rows, cols, sr, sc,
-                       codes, scales);
+    constexpr int DT = decltype(dt)::value;
+    auto k = sc == 1 ? mx_quantize_kernel<DT, true> : mx_quantize_kernel<DT, false>;
+    hipLaunchKernelGGL(k, dim3(tiles), dim3(256), 0, st,
+                       static_cast<const typename Elem<DT>::type*>(x), rows, cols, sr, sc, codes,
+                       scales);
   });
   HIP_TRY(hipGetLastError());
 }
 
-// Which kernel a product of I x J outputs takes: the largest tile that leaves
-// most of the 256 CUs one, and with fewer tiles the kernel that splits the depth
-// over a block's waves.  fp4, us: 16384 x 8192 x 8192 665 on 256 x 256 tiles, 719
-// on 128 x 128; 1001 x 300 x 400 14.0 on 128 x 128 tiles, 6.7 split.  bf16: 8192 x 4096
-// x 4096 207 against 268, 1001 x 400 x 3 planes of 300 28.4 against 11.0.
+// Which kernel products take: the largest tile that leaves most of the 256 CUs
+// one, and with fewer tiles the kernel that splits the depth over a block's
+// waves.  fp4, us: 16384 x 8192 x 8192 498 on 256 x 256 tiles, 695 on 128 x 128; 1001 x
+// 300 x 400 14.0 on 128 x 128 tiles, 6.7 split.  bf16: 8192 x 4096 x 4096 186 against
+// 250, 1001 x 400 x 3 planes of 300 28.4 against 11.0.
+enum { MX_BIG, MX_MID, MX_SPLIT, MX_ROWS16 };
+static long long mx_tiles(int I, int J, int t) {
+  return (long long)ceil_div(I, t) * ceil_div(J, t);
+}
+static int mx_pick(long long big, long long mid) {
+  return big >= 200 ? MX_BIG : mid >= 128 ? MX_MID : MX_SPLIT;
+}
+
 template <bool FP4>
-static void mx_gemm_launch(hipStream_t st, MxGemm g) {
-  MxOut& o = g.o;
-  if (!o.I || !o.J) return;
-  const int es = elem_size(o.dtype);
-  o.vec = o.ldo * es % 16 == 0 && aligned16(o.y);
-  const long long big = (long long)ceil_div(o.I, 256) * ceil_div(o.J, 256);
-  const long long mid = (long long)ceil_div(o.I, 128) * ceil_div(o.J, 128);
-  if (big >= 200) {
-    hipLaunchKernelGGL((mx_tile_kernel<FP4, 2, 4, 8, 4, 4>), dim3(grid_x(big)), dim3(512), 0, st, g);
-  } else if (mid >= 128) {
-    hipLaunchKernelGGL((mx_tile_kernel<FP4, 2, 2, 4, 4, 4>), dim3(grid_x(mid)), dim3(256), 0, st, g);
-  } else if (o.I <= 16) {
-    hipLaunchKernelGGL((mx_split_kernel<FP4, 1, 1, 8>), dim3(ceil_div(o.J, 16)), dim3(512), 0, st,
-                       g);
-  } else {
-    const long long small = (long long)ceil_div(o.I, 64) * ceil_div(o.J, 64);
-    hipLaunchKernelGGL((mx_split_kernel<FP4, 4, 4, 4>), dim3(grid_x(small)), dim3(256), 0, st, g);
+static void mx_gemm_launch(hipStream_t st, MxGemms& p, int pick) {
+  auto launch = [&](auto k, int tile, int threads) {
+    long long n = 0;
+    for (int i = 0; i < 2; ++i) {
+      MxOut& o = p.g[i].o;
+      if (i < p.n) {
+        o.vec = o.ldo * elem_size(o.dtype) % 16 == 0 && aligned16(o.y);
+        n += mx_tiles(o.I, o.J, tile);
+      }
+      p.end[i] = (int)grid_x(n);
+    }
+    n += ceil_div(p.db_n, 64);
+    if (!n) return;
+    hipLaunchKernelGGL(k, dim3(grid_x(n)), dim3(threads), 0, st, p);
+    HIP_TRY(hipGetLastError());
+  };
+  switch (pick) {
+    case MX_BIG: launch(mx_tile_kernel<FP4, 2, 4, 8, 4, 4>, 256, 512); break;
+    case MX_MID: launch(mx_tile_kernel<FP4, 2, 2, 4, 4, 4>, 128, 256); break;
+    case MX_SPLIT: launch(mx_split_kernel<FP4, 4, 4, 4>, 64, 256); break;
+    default:
+      if constexpr (FP4) launch(mx_split_kernel<true, 1, 1, 8>, 16, 512);
   }
-  HIP_TRY(hipGetLastError());
 }
 
 static FragOp mx_op(const MxMat& q) {
@@ -240,7 +299,12 @@ static FragOp mx_op(const MxMat& q) {
 }
 
 void mx_linear_launch(hipStream_t st, const MxMat& x, const MxMat& w, const MxOut& o) {
-  mx_gemm_launch<true>(st, MxGemm{mx_op(x), mx_op(w), x.kt(), 1, o});
+  MxGemms p{};
+  if (!o.I || !o.J) return;
+  p.n = 1;
+  p.g[0] = {mx_op(x), mx_op(w), x.kt(), 1, o};
+  mx_gemm_launch<true>(st, p, o.I <= 16 ? MX_ROWS16
+                                        : mx_pick(mx_tiles(o.I, o.J, 256), mx_tiles(o.I, o.J, 128)));
 }
 
 // The gradient's workspace, in order.
@@ -268,50 +332,53 @@ static MxGradWs mx_grad_ws(int dtype, int M, int N, int K, bool dx, bool dw, boo
   return w;
 }
 
-static void mx_turn(hipStream_t st, const MxMat& q, uint8_t* out) {
-  if (!q.rows || !q.cols) return;
-  hipLaunchKernelGGL(mx_turn_kernel, dim3(grid_x((long long)q.kt() * ceil_div(q.rows, 64))),
-                     dim3(256), 0, st, q, out);
-  HIP_TRY(hipGetLastError());
-}
-
-static void mx_plane_gemm(hipStream_t st, const uint8_t* A, const uint8_t* B, int I, int J,
-                          int steps, int planes, void* C, int dtype) {
-  const MxOut o{C, nullptr, J, I, J, dtype, 0, DDPG_ACT_NONE, 0};
-  mx_gemm_launch<false>(st, MxGemm{{A, nullptr, ceil_div(I, 64) * 4},
-                                   {B, nullptr, ceil_div(J, 64) * 4}, steps, planes, o});
-}
-
 void mx_linear_grad_launch(hipStream_t st, int dtype, const void* dy, long long sr, long long sc,
                            const MxMat& x, const MxMat& w, void* dx, float* dw, float* db,
                            uint8_t* ws) {
   const int M = x.rows, N = w.rows, K = x.cols;
   const MxGradWs L = mx_grad_ws(dtype, M, N, K, dx, dw, db);
-  uint8_t* flat = dx ? ws + L.flat : nullptr;
-  uint8_t* turned = dw ? ws + L.turned : nullptr;
-  float* part = db ? reinterpret_cast<float*>(ws + L.part) : nullptr;
-  if (M && N && (dx || dw || db)) {
+  MxPrep a{};
+  a.dy = dy;
+  a.sr = sr;
+  a.sc = sc;
+  a.M = M;
+  a.N = N;
+  a.w = w;
+  a.x = x;
+  a.flat = dx ? ws + L.flat : nullptr;
+  a.turned = dw ? ws + L.turned : nullptr;
+  a.part = db ? reinterpret_cast<float*>(ws + L.part) : nullptr;
+  a.wt = ws + L.wt;
+  a.xt = ws + L.xt;
+  const long long n64 = ceil_div(N, 64), m64 = ceil_div(M, 64), kt = ceil_div(K, 128);
+  const long long nd = (dx || dw || db) ? n64 * m64 : 0, nw = dx ? n64 * kt : 0,
+                  nx = dw ? m64 * kt : 0;
+  a.dy_blocks = (int)grid_x(nd);
+  a.w_blocks = (int)grid_x(nw);
+  if (nd + nw + nx)
     by_dtype(dtype, [&](auto dt) {
-      hipLaunchKernelGGL((mx_dy_kernel<dt.value, mx_planes(dt.value)>),
-                         dim3(grid_x((long long)ceil_div(N, 64) * ceil_div(M, 64))), dim3(256), 0,
-                         st, static_cast<const typename Elem<dt.value>::type*>(dy), sr, sc, M, N,
-                         flat, turned, part);
+      hipLaunchKernelGGL(mx_prep_kernel<decltype(dt)::value>, dim3(grid_x(nd + nw + nx)), dim3(256),
+                         0, st, a);
     });
-    HIP_TRY(hipGetLastError());
-  }
-  if (db && N) {
-    hipLaunchKernelGGL(mx_db_kernel, dim3(ceil_div(N, 256)), dim3(256), 0, st, part,
-                       ceil_div(M, 64), N, db);
-    HIP_TRY(hipGetLastError());
-  }
-  if (dx) {
-    mx_turn(st, w, ws + L.wt);
-    mx_plane_gemm(st, flat, ws + L.wt, M, K, L.sn, L.P, dx, dtype);
-  }
-  if (dw) {
-    mx_turn(st, x, ws + L.xt);
-    mx_plane_gemm(st, turned, ws + L.xt, N, K, L.sm, L.P, dw, T_FP32);
-  }
+  HIP_TRY(hipGetLastError());
+  MxGemms p{};
+  auto add = [&](const uint8_t* I, const uint8_t* J, int ni, int nj, int steps, void* C, int type) {
+    if (!ni || !nj) return;
+    p.g[p.n++] = {{I, nullptr, ceil_div(ni, 64) * 4},
+                  {J, nullptr, ceil_div(nj, 64) * 4},
+                  steps,
+                  L.P,
+                  {C, nullptr, nj, ni, nj, type, 0, DDPG_ACT_NONE, 0}};
+  };
+  if (dx) add(a.flat, a.wt, M, K, L.sn, dx, dtype);
+  if (dw) add(a.turned, a.xt, N, K, L.sm, dw, T_FP32);
+  p.db = db;
+  p.db_part = a.part;
+  p.db_n = db ? N : 0;
+  p.db_parts = (int)m64;
+  // by both products' tiles, so that a result does not depend on which are asked
+  mx_gemm_launch<false>(st, p, mx_pick(mx_tiles(M, K, 256) + mx_tiles(N, K, 256),
+                                       mx_tiles(M, K, 128) + mx_tiles(N, K, 128)));
 }
 
 }  // namespace ddpg
@@ -348,11 +415,12 @@ int ddpg_mx_dequantize(int device, void* stream, const void* codes, const void* 
     if (!out) throw einval("mx_dequantize: null output");
     if (row_stride < cols) throw einval("mx_dequantize: rows %lld apart overlap", (long long)row_stride);
     OnDevice on(device);
-    const long long tiles = (long long)ceil_div(q.rows, 16) * q.kt();
+    const unsigned tiles = grid_x((long long)ceil_div(q.rows, 64) * q.kt());
     by_dtype(dtype, [&](auto dt) {
-      hipLaunchKernelGGL(mx_dequantize_kernel<dt.value>, dim3(grid_x((tiles + 3) / 4)), dim3(256), 0,
+      constexpr int DT = decltype(dt)::value;
+      hipLaunchKernelGGL(mx_dequantize_kernel<DT>, dim3(tiles), dim3(256), 0,
                          static_cast<hipStream_t>(stream), q,
-                         static_cast<typename Elem<dt.value>::type*>(out), (long long)row_stride);
+                         static_cast<typename Elem<DT>::type*>(out), (long long)row_stride);
     });
     HIP_TRY(hipGetLastError());
   });

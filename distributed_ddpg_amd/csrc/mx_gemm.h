@@ -37,6 +37,16 @@ struct MxGemm {
   MxOut o;
 };
 
+// One launch: n products (blocks 0 .. end[0] - 1, .. end[1] - 1), then 64 columns
+// a block of a bias gradient's last sum.
+struct MxGemms {
+  MxGemm g[2];
+  int n, end[2];
+  const float* db_part;  // [db_parts][db_n]
+  float* db;
+  int db_parts, db_n;
+};
+
 DDPG_DEV float mx_act(float v, int act) {
   if (act == DDPG_ACT_ELU) return elu_f(v);
   if (act == DDPG_ACT_TANH) return tanhf(v);
@@ -132,12 +142,28 @@ DDPG_DEV f32x4 frag_mfma(const u32x4& j, const u32x4& i, f32x4 acc, unsigned sj,
                                                    __builtin_bit_cast(bf16x8, i), acc, 0, 0, 0);
 }
 
-// Tile of a block.  The grid is one-dimensional: every XCD (workgroups are
+// db[n] = the sum of the row blocks' column sums, in float64: the launch's last
+// blocks, 64 columns each, the waves taking partials in turn.
+template <int NW>
+DDPG_DEV void mx_db(const MxGemms& p, int b, double (&red)[NW][64]) {
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, n = b * 64 + l;
+  double s = 0;
+  if (n < p.db_n)
+#pragma unroll 4
+    for (int i = w; i < p.db_parts; i += NW) s += p.db_part[(size_t)i * p.db_n + n];
+  red[w][l] = s;
+  __syncthreads();
+  if (w || n >= p.db_n) return;
+  for (int i = 1; i < NW; ++i) s += red[i][l];
+  p.db[n] = (float)s;
+}
+
+// Tile `lin` of a product.  The grid is one-dimensional: every XCD (workgroups are
 // dealt to the 8 in turn) takes a contiguous run of the order, which walks
 // eight rows of tiles down before it steps across, so that the tiles an XCD
 // works on at once share their operands in its L2.
-DDPG_DEV void tile_of(int ni, int nj, int& ti, int& tj) {
-  const int n = ni * nj, lin = blockIdx.x;
+DDPG_DEV void tile_of(int lin, int ni, int nj, int& ti, int& tj) {
+  const int n = ni * nj;
   const int x = lin & 7, q = n >> 3, r = n & 7;
   const int t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (lin >> 3);
   const int band = t / (8 * nj), in = t - band * 8 * nj;
@@ -196,16 +222,22 @@ struct RingCfg {
 // drain the loads in flight before reads of its own; the wait that ends the step
 // is tied to their registers, so none is touched while a read is under way.
 template <bool FP4, int WI, int WJ, int TI, int TJ, int NS>
-__global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemm g) {
+__global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
   using C = RingCfg<FP4, WI, WJ, TI, TJ, NS>;
   __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
+  if ((int)blockIdx.x >= p.end[1]) {
+    mx_db<C::NW>(p, blockIdx.x - p.end[1], *reinterpret_cast<double(*)[C::NW][64]>(smem));
+    return;
+  }
+  const bool second = (int)blockIdx.x >= p.end[0];
+  const MxGemm& g = p.g[second];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ, wj = wave % WJ;
   const int ni = (g.o.I + C::GI * 16 - 1) / (C::GI * 16);
   const int nj = (g.o.J + C::GJ * 16 - 1) / (C::GJ * 16);
   int ti, tj;
-  tile_of(ni, nj, ti, tj);
+  tile_of(blockIdx.x - (second ? p.end[0] : 0), ni, nj, ti, tj);
   const int nk = g.kt * g.planes;
 
   // this wave's pieces of a step: source of the next step to load, LDS place.
@@ -373,13 +405,19 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemm g) {
 // with operands straight from memory, two steps ahead; the waves' sums are
 // joined in LDS in wave order.
 template <bool FP4, int TI, int TJ, int NW>
-__global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemm g) {
+__global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemms p) {
   __shared__ f32x4 part[NW][TI * TJ][64];
+  if ((int)blockIdx.x >= p.end[1]) {
+    mx_db<NW>(p, blockIdx.x - p.end[1], *reinterpret_cast<double(*)[NW][64]>(part));
+    return;
+  }
+  const bool second = (int)blockIdx.x >= p.end[0];
+  const MxGemm& g = p.g[second];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ni = (g.o.I + TI * 16 - 1) / (TI * 16), nj = (g.o.J + TJ * 16 - 1) / (TJ * 16);
   int ti, tj;
-  tile_of(ni, nj, ti, tj);
+  tile_of(blockIdx.x - (second ? p.end[0] : 0), ni, nj, ti, tj);
   const int nk = g.kt * g.planes;
   f32x4 acc[TI][TJ];
 #pragma unroll
