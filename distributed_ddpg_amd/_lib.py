@@ -73,8 +73,6 @@ _dp = ctypes.POINTER(ctypes.c_double)
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _u8p = ctypes.POINTER(ctypes.c_uint8)
 _u32p = ctypes.POINTER(ctypes.c_uint32)
-_ip = ctypes.POINTER(ctypes.c_int)
-_PP = ctypes.POINTER(ctypes.c_void_p)
 _szp = ctypes.POINTER(ctypes.c_size_t)
 _i64 = ctypes.c_int64
 
@@ -127,10 +125,10 @@ PROTOTYPES = [
     ("ddpg_profile_enable", _c.c_int, [_P, _c.c_int]),
     ("ddpg_profile_read", _c.c_int, [_P, _c.c_int, _P, _dp, _i64p, _dp, _dp]),
     ("ddpg_global_norm_workspace", _c.c_size_t, [_c.c_int]),
-    ("ddpg_global_norm", _c.c_int, [_c.c_int, _P, _c.c_int, _ip, _PP, _i64p, _i64p, _i64p, _P,
-                                    _c.c_size_t, _P]),
-    ("ddpg_clip_by_global_norm", _c.c_int, [_c.c_int, _P, _c.c_int, _ip, _PP, _PP, _i64p, _i64p,
-                                            _i64p, _c.c_float, _P, _P, _c.c_size_t, _P]),
+    ("ddpg_global_norm", _c.c_int, [_c.c_int, _P, _c.c_int, _P, _P, _P, _P, _P, _P, _c.c_size_t,
+                                    _P]),
+    ("ddpg_clip_by_global_norm", _c.c_int, [_c.c_int, _P, _c.c_int, _P, _P, _P, _P, _P, _P,
+                                            _c.c_float, _P, _P, _c.c_size_t, _P]),
     ("ddpg_mx_sizes", _c.c_int, [_i64, _i64, _szp, _szp]),
     ("ddpg_mx_quantize", _c.c_int, [_c.c_int, _P, _c.c_int, _P, _i64, _i64, _i64, _i64, _P, _P]),
     ("ddpg_mx_dequantize", _c.c_int, [_c.c_int, _P, _P, _P, _i64, _i64, _c.c_int, _P, _i64]),

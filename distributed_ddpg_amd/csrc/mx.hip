@@ -24,18 +24,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(
   unsigned s = 0;
   if (g64 * 64 + (r & ~15) < rows) {
     float v[32];
-    const typename Elem<DT>::type* p = x + min(row, rows - 1) * sr;
-    if (ROWS && c0 + 32 <= cols) {
-      constexpr int V = Elem<DT>::V;
-#pragma unroll
-      for (int i = 0; i < 32; i += V)
-        Elem<DT>::widen(*reinterpret_cast<const U16B*>(p + c0 + i), v + i);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = (float)p[min(c0 + i, cols - 1) * sc];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = c0 + i < cols ? v[i] : 0.f;
-    }
+    mx_load_block<DT>(x + min(row, rows - 1) * sr, sc, ROWS, c0, cols, v);
     const u32x4 q = mx_quantize_block(v, s);
     *reinterpret_cast<u32x4*>(codes + mx_code_at(g64 * 4 + (r >> 4), kt, k) +
                               (kb * 16 + (r & 15)) * 16) = q;
@@ -260,6 +249,10 @@ void mx_quantize_launch(hipStream_t st, int dtype, const void* x, int rows, int 
 // waves.  fp4, us: 16384 x 8192 x 8192 498 on 256 x 256 tiles, 695 on 128 x 128; 1001 x
 // 300 x 400 14.0 on 128 x 128 tiles, 6.7 split.  bf16: 8192 x 4096 x 4096 186 against
 // 250, 1001 x 400 x 3 planes of 300 28.4 against 11.0.
+static bool mx_rows_aligned(const MxOut& o) {
+  return o.ldo * elem_size(o.dtype) % 16 == 0 && aligned16(o.y);
+}
+
 enum { MX_BIG, MX_MID, MX_SPLIT, MX_ROWS16 };
 static long long mx_tiles(int I, int J, int t) {
   return (long long)ceil_div(I, t) * ceil_div(J, t);
@@ -275,7 +268,7 @@ static void mx_gemm_launch(hipStream_t st, MxGemms& p, int pick) {
     for (int i = 0; i < 2; ++i) {
       MxOut& o = p.g[i].o;
       if (i < p.n) {
-        o.vec = o.ldo * elem_size(o.dtype) % 16 == 0 && aligned16(o.y);
+        o.vec = mx_rows_aligned(o);
         n += mx_tiles(o.I, o.J, tile);
       }
       p.end[i] = (int)grid_x(n);
@@ -305,6 +298,19 @@ void mx_linear_launch(hipStream_t st, const MxMat& x, const MxMat& w, const MxOu
   p.g[0] = {mx_op(x), mx_op(w), x.kt(), 1, o};
   mx_gemm_launch<true>(st, p, o.I <= 16 ? MX_ROWS16
                                         : mx_pick(mx_tiles(o.I, o.J, 256), mx_tiles(o.I, o.J, 128)));
+}
+
+// at most 16 rows, quantised on the way
+void mx_linear_rows_launch(hipStream_t st, int dtype, const void* x, long long sr, long long sc,
+                           int M, int K, const MxMat& w, MxOut o) {
+  if (!M || !o.J) return;
+  o.vec = mx_rows_aligned(o);
+  const RawX r{x, sr, sc, M, K, dtype, sc == 1};
+  by_dtype(dtype, [&](auto dt) {
+    hipLaunchKernelGGL((mx_rows_kernel<decltype(dt)::value, 8>), dim3(ceil_div(o.J, 16)), dim3(512),
+                       0, st, r, mx_op(w), w.kt(), o);
+  });
+  HIP_TRY(hipGetLastError());
 }
 
 // The gradient's workspace, in order.
@@ -370,8 +376,11 @@ void mx_linear_grad_launch(hipStream_t st, int dtype, const void* dy, long long 
                   L.P,
                   {C, nullptr, nj, ni, nj, type, 0, DDPG_ACT_NONE, 0}};
   };
+  // the deeper product's tiles first: the shorter ones fill in behind them
+  const bool dw_first = L.sm > L.sn;
+  if (dw && dw_first) add(a.turned, a.xt, N, K, L.sm, dw, T_FP32);
   if (dx) add(a.flat, a.wt, M, K, L.sn, dx, dtype);
-  if (dw) add(a.turned, a.xt, N, K, L.sm, dw, T_FP32);
+  if (dw && !dw_first) add(a.turned, a.xt, N, K, L.sm, dw, T_FP32);
   p.db = db;
   p.db_part = a.part;
   p.db_n = db ? N : 0;
@@ -431,7 +440,8 @@ int ddpg_mx_linear(int device, void* stream, int x_dtype, const void* x, int64_t
                    const void* w_codes, const void* w_scales, int64_t N, int bias_dtype,
                    const void* bias, int act, int dtype, void* y, int64_t y_row_stride) {
   return guard(nullptr, [&] {
-    const MxMat xq = mx_mat("mx_linear x", x_codes, x_scales, M, K);
+    const bool rows = x && M <= 16;  // needs no scratch
+    const MxMat xq = mx_mat("mx_linear x", x_codes, x_scales, M, rows ? 0 : K);
     const MxMat wq = mx_mat("mx_linear w", w_codes, w_scales, N, K);
     check_dtype("mx_linear", dtype);
     if (x) check_dtype("mx_linear x", x_dtype);
@@ -442,10 +452,14 @@ int ddpg_mx_linear(int device, void* stream, int x_dtype, const void* x, int64_t
     if (y_row_stride < N) throw einval("mx_linear: rows %lld apart overlap", (long long)y_row_stride);
     OnDevice on(device);
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    const MxOut o{y, bias, (long long)y_row_stride, (int)M, (int)N, dtype, bias_dtype, act, 0};
+    if (rows) {
+      mx_linear_rows_launch(st, x_dtype, x, x_row_stride, x_col_stride, (int)M, (int)K, wq, o);
+      return;
+    }
     if (x)
       mx_quantize_launch(st, x_dtype, x, (int)M, (int)K, x_row_stride, x_col_stride,
                          static_cast<uint8_t*>(x_codes), static_cast<uint8_t*>(x_scales));
-    const MxOut o{y, bias, (long long)y_row_stride, (int)M, (int)N, dtype, bias_dtype, act, 0};
     mx_linear_launch(st, xq, wq, o);
   });
 }

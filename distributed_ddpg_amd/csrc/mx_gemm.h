@@ -404,6 +404,63 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
 // One block: TI x TJ fragments of C, its NW waves taking every NW-th depth step
 // with operands straight from memory, two steps ahead; the waves' sums are
 // joined in LDS in wave order.
+// Up to 16 rows of x as they are: the block's products quantise them on their way
+// to the registers (each block again: x is small and stays in the caches, and a
+// launch is saved).
+struct RawX {
+  const void* p;
+  long long sr, sc;
+  int rows, cols, dtype;
+  int vec;  // columns adjacent
+};
+
+template <int DT>
+DDPG_DEV void mx_load_block(const typename Elem<DT>::type* p, long long sc, bool adjacent, int c0,
+                            int cols, float (&v)[32]) {
+  if (adjacent && c0 + 32 <= cols) {
+    constexpr int V = Elem<DT>::V;
+#pragma unroll
+    for (int i = 0; i < 32; i += V)
+      Elem<DT>::widen(*reinterpret_cast<const U16B*>(p + c0 + i), v + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = (float)p[min(c0 + i, cols - 1) * sc];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = c0 + i < cols ? v[i] : 0.f;
+  }
+}
+
+// y = act(x w^T + b) for at most 16 rows: a block makes 16 columns, its waves
+// taking every NW-th depth step, the sums joined in wave order.
+template <int DT, int NW>
+__global__ __launch_bounds__(64 * NW) void mx_rows_kernel(RawX x, FragOp w, int kt, MxOut o) {
+  __shared__ f32x4 part[NW][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, gj = blockIdx.x;
+  const typename Elem<DT>::type* xp =
+      static_cast<const typename Elem<DT>::type*>(x.p) + min(lane & 15, x.rows - 1) * x.sr;
+  const uint8_t* pj = w.p + (size_t)gj * kt * 1024 + lane * 16;
+  const uint8_t* qj = w.scales + (size_t)(gj >> 2) * kt * 256 + lane * 4 + (gj & 3);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s = wave; s < kt; s += NW) {
+    const u32x4 j = *reinterpret_cast<const u32x4*>(pj + (size_t)s * 1024);
+    const unsigned sj = qj[(size_t)s * 256];
+    // rows past x's repeat its last one, their results are not stored
+    float v[32];
+    mx_load_block<DT>(xp, x.sc, x.vec, s * 128 + (lane >> 4) * 32, x.cols, v);
+    unsigned si;
+    const u32x4 i = mx_quantize_block(v, si);
+    acc = mx_mfma<0, 0>(j, i, acc, sj, si);
+  }
+  part[wave][lane] = acc;
+  __syncthreads();
+  if (wave) return;
+  for (int s = 1; s < NW; ++s) acc += part[s][lane];
+  const int jj = gj * 16 + (lane >> 4) * 4;
+  float b[4];
+  mx_bias(o, jj, b);
+  mx_store(o, lane & 15, jj, acc, b);
+}
+
 template <bool FP4, int TI, int TJ, int NW>
 __global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemms p) {
   __shared__ f32x4 part[NW][TI * TJ][64];

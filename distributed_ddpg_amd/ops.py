@@ -17,7 +17,7 @@ tensor that requires grad is refused while grad mode is on.  Arguments of the
 wrong shape, type or device raise ValueError, the library's own refusals
 DDPGError.
 """
-import ctypes
+from array import array
 
 import torch
 
@@ -33,8 +33,8 @@ def _check(rc):
         raise _lib.DDPGError(rc, (lib.ddpg_global_error() or b"").decode(errors="replace"))
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+# the raw handle of torch's current stream on a device ordinal
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _tensor(name, t):
@@ -83,58 +83,50 @@ def _rows(t):
 class _List:
     """The C form of a tensor list (None entries dropped)."""
 
-    def __init__(self, name, tensors, inplace):
-        self.kept = [t for t in tensors if t is not None]
-        self.src, dt, cols, ld = [], [], [], []
-        self.device = None
-        strided = False
-        for i, t in enumerate(self.kept):
-            dt.append(_tensor("%s[%d]" % (name, i), t))
-            if self.device is None:
-                self.device = t.device
-            elif t.device != self.device:
-                raise ValueError("%s: tensors on %s and %s" % (name, self.device, t.device))
-            if not t.is_contiguous():
+    def __init__(self, tensors, inplace):
+        self.src = src = [t for t in tensors if t is not None]
+        if not src:
+            raise ValueError("t_list: no tensor in the list")
+        dt = array("i", [_tensor("t_list", t) for t in src])
+        self.index = src[0].get_device()
+        for t in src:
+            if t.get_device() != self.index:
+                raise ValueError("t_list: tensors on %s and %s" % (src[0].device, t.device))
+        self.kept = src
+        cols = ld = None
+        if not all([t.is_contiguous() for t in src]):
+            self.src = src = list(src)
+            cols, ld = array("q", bytes(8 * len(src))), array("q", bytes(8 * len(src)))
+            for i, t in enumerate(src):
                 rc = _rows(t)
+                if rc is None and inplace:
+                    raise ValueError("t_list[%d]: strides %s are neither dense nor evenly spaced "
+                                     "rows" % (i, tuple(t.stride())))
                 if rc is None:
-                    if inplace:
-                        raise ValueError("%s[%d]: strides %s are neither dense nor evenly spaced "
-                                         "rows" % (name, i, tuple(t.stride())))
-                    t, rc = t.contiguous(), (0, 0)
-                strided = strided or rc[0] > 0
-                cols.append(rc[0])
-                ld.append(rc[1])
-            else:
-                cols.append(0)
-                ld.append(0)
-            self.src.append(t)
-        n = self.n = len(self.src)
-        self.dtype = (ctypes.c_int * n)(*dt)
-        self.ptr = (ctypes.c_void_p * n)(*[t.data_ptr() for t in self.src])
-        self.count = (ctypes.c_int64 * n)(*[t.numel() for t in self.src])
-        self.cols = (ctypes.c_int64 * n)(*cols) if strided else None
-        self.ld = (ctypes.c_int64 * n)(*ld) if strided else None
+                    src[i] = t.contiguous()
+                else:
+                    cols[i], ld[i] = rc
+        self.cols = cols
+        self.ptr = array("Q", [t.data_ptr() for t in src])
+        self._held = (dt, cols, ld, array("q", [t.numel() for t in src]))
+        self.n = len(src)
+        addr = lambda a: None if a is None else a.buffer_info()[0]
+        self.dtype, cols, ld, self.count = [addr(a) for a in self._held]
+        self.rows = (cols, ld)
+        self.ws_bytes = lib.ddpg_global_norm_workspace(self.n)
 
-    def need_device(self, name):
-        if self.device is None:
-            raise ValueError("%s: no tensor in the list" % name)
-        return self.device
-
-    def workspace(self):
-        nb = lib.ddpg_global_norm_workspace(self.n)
-        return torch.empty(nb, dtype=torch.uint8, device=self.device), nb
+    def empty(self, n, dtype):
+        return torch.empty(n, dtype=dtype, device=self.kept[0].device)
 
 
 def global_norm(t_list):
     """sqrt of the sum of all elements' squares, a float32 scalar tensor.
     The sum runs in float64 in a fixed order.  Tensors may mix float32, bfloat16
     and float16 and be of any strides; None entries count nothing."""
-    l = _List("t_list", t_list, False)
-    dev = l.need_device("t_list")
-    ws, nb = l.workspace()
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    _check(lib.ddpg_global_norm(dev.index, _stream(dev), l.n, l.dtype, l.ptr, l.count, l.cols,
-                                l.ld, ws.data_ptr(), nb, norm.data_ptr()))
+    l = _List(t_list, False)
+    norm, ws = l.empty((), torch.float32), l.empty(l.ws_bytes, torch.uint8)
+    _check(lib.ddpg_global_norm(l.index, _stream(l.index), l.n, l.dtype, l.ptr.buffer_info()[0],
+                                l.count, *l.rows, ws.data_ptr(), l.ws_bytes, norm.data_ptr()))
     return norm
 
 
@@ -151,26 +143,24 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, inplace=False):
     clip_norm = float(clip_norm)
     if not clip_norm >= 0:
         raise ValueError("clip_norm %r is not a number >= 0" % clip_norm)
-    l = _List("t_list", t_list, inplace)
-    dev = l.need_device("t_list")
+    l = _List(t_list, inplace)
     if use_norm is not None:
         if _tensor("use_norm", use_norm) != _lib.FP32 or use_norm.numel() != 1 or (
-                use_norm.device != dev):
-            raise ValueError("use_norm: expected one float32 on %s" % dev)
-        norm, ws, nb = use_norm, None, 0
+                use_norm.get_device() != l.index):
+            raise ValueError("use_norm: expected one float32 on %s" % l.kept[0].device)
+        norm, wp, nb, given, to = use_norm, None, 0, use_norm.data_ptr(), None
     else:
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        ws, nb = l.workspace()
+        norm, ws, nb = l.empty((), torch.float32), l.empty(l.ws_bytes, torch.uint8), l.ws_bytes
+        wp, given, to = ws.data_ptr(), None, norm.data_ptr()
     if inplace:
         out, dst = l.kept, l.ptr
     else:
-        out = [torch.empty(t.shape, dtype=t.dtype, device=dev) if l.cols and l.cols[i]
+        out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if l.cols and l.cols[i]
                else torch.empty_like(t) for i, t in enumerate(l.src)]
-        dst = (ctypes.c_void_p * l.n)(*[t.data_ptr() for t in out])
+        dst = array("Q", [t.data_ptr() for t in out])
     _check(lib.ddpg_clip_by_global_norm(
-        dev.index, _stream(dev), l.n, l.dtype, l.ptr, dst, l.count, l.cols, l.ld, clip_norm,
-        None if use_norm is None else norm.data_ptr(), None if ws is None else ws.data_ptr(), nb,
-        None if use_norm is not None else norm.data_ptr()))
+        l.index, _stream(l.index), l.n, l.dtype, l.ptr.buffer_info()[0], dst.buffer_info()[0],
+        l.count, *l.rows, clip_norm, given, wp, nb, to))
     it = iter(out)
     return [None if t is None else next(it) for t in t_list], norm
 
@@ -178,17 +168,16 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, inplace=False):
 # ---------------------------------------------------------------- MXFP4
 class MXTensor:
     """A [rows, cols] matrix in MXFP4: 4-bit codes and a scale byte for 32 of
-    them along a row, in the order the matrix instructions read (an opaque pair
-    of byte buffers; .dequantize() gives the values).  17/32 byte a value."""
+    them along a row, in the order the matrix instructions read (an opaque buffer;
+    .dequantize() gives the values).  17/32 byte a value."""
 
-    __slots__ = ("codes", "scales", "shape")
+    __slots__ = ("buffer", "shape", "device", "_index", "_codes", "_scales")
 
-    def __init__(self, codes, scales, shape):
-        self.codes, self.scales, self.shape = codes, scales, shape
-
-    @property
-    def device(self):
-        return self.codes.device
+    def __init__(self, buffer, shape):
+        self.buffer, self.shape = buffer, shape
+        self.device, self._index = buffer.device, buffer.get_device()
+        self._codes = buffer.data_ptr()  # the scales come behind the codes
+        self._scales = self._codes + buffer.numel() // 17 * 16
 
     def dequantize(self, dtype=torch.float32):
         return mx_dequantize(self, dtype)
@@ -204,21 +193,19 @@ def _matrix(name, t):
     return code
 
 
-def _mx(name, q, cols=None, device=None):
+def _mx(name, q, cols=None, index=None):
     if not isinstance(q, MXTensor):
         raise ValueError("%s: expected an MXTensor (mx_quantize), got %s" % (name,
                                                                             type(q).__name__))
     if cols is not None and q.shape[1] != cols:
-        raise ValueError("%s: expected [*, %d], got %s" % (name, cols, tuple(q.shape)))
-    if device is not None and q.device != device:
-        raise ValueError("%s is on %s, the other operand on %s" % (name, q.device, device))
+        raise ValueError("%s: expected [*, %d], got %s" % (name, cols, q.shape))
+    if index is not None and q._index != index:
+        raise ValueError("%s is on %s, not with the other operands" % (name, q.device))
     return q
 
 
-def _mx_empty(rows, cols, device):
-    tiles = -(-rows // 64) * -(-cols // 128)
-    buf = torch.empty(tiles * 4352, dtype=torch.uint8, device=device)
-    return MXTensor(buf[:tiles * 4096], buf[tiles * 4096:], (rows, cols))
+def _mx_bytes(rows, cols):
+    return -(-rows // 64) * -(-cols // 128) * 4352
 
 
 def mx_quantize(x):
@@ -229,10 +216,11 @@ def mx_quantize(x):
     the even code, larger ones 6.  A block that holds an infinity or a NaN is
     NaN as a whole."""
     code = _matrix("x", x)
-    q = _mx_empty(x.shape[0], x.shape[1], x.device)
-    _check(lib.ddpg_mx_quantize(x.device.index, _stream(x.device), code, x.data_ptr(), x.shape[0],
-                                x.shape[1], x.stride(0), x.stride(1), q.codes.data_ptr(),
-                                q.scales.data_ptr()))
+    (rows, cols), (s0, s1) = x.shape, x.stride()
+    q = MXTensor(torch.empty(_mx_bytes(rows, cols), dtype=torch.uint8, device=x.device),
+                 (rows, cols))
+    _check(lib.ddpg_mx_quantize(q._index, _stream(q._index), code, x.data_ptr(), rows, cols, s0,
+                                s1, q._codes, q._scales))
     return q
 
 
@@ -243,9 +231,8 @@ def mx_dequantize(q, dtype=torch.float32):
     if dtype not in _DTYPES:
         raise ValueError("dtype: %s is none of float32, bfloat16, float16" % dtype)
     out = torch.empty(q.shape, dtype=dtype, device=q.device)
-    _check(lib.ddpg_mx_dequantize(q.device.index, _stream(q.device), q.codes.data_ptr(),
-                                  q.scales.data_ptr(), q.shape[0], q.shape[1], _DTYPES[dtype],
-                                  out.data_ptr(), q.shape[1]))
+    _check(lib.ddpg_mx_dequantize(q._index, _stream(q._index), q._codes, q._scales, q.shape[0],
+                                  q.shape[1], _DTYPES[dtype], out.data_ptr(), q.shape[1]))
     return out
 
 
@@ -255,36 +242,41 @@ def mx_linear(x, w, bias=None, act=None, dtype=None):
     float32; the result is of x's type, or of dtype (float32 if x is an
     MXTensor)."""
     _mx("w", w)
-    N, K = w.shape
-    dev = w.device
+    (N, K), index = w.shape, w._index
     if act not in _ACTS:
         raise ValueError("act: %r is none of None, 'elu', 'tanh'" % (act,))
     if isinstance(x, MXTensor):
-        xq, xp, xc, s0, s1 = _mx("x", x, K, dev), None, 0, 0, 0
+        _mx("x", x, K, index)
+        M, xp, xc, s0, s1, codes, scales = x.shape[0], None, 0, 0, 0, x._codes, x._scales
         dtype = dtype or torch.float32
     else:
         xc = _matrix("x", x)
-        if x.shape[1] != K:
+        M, k = x.shape
+        if k != K:
             raise ValueError("x: expected [*, %d], got %s" % (K, tuple(x.shape)))
-        if x.device != dev:
-            raise ValueError("x is on %s, w on %s" % (x.device, dev))
-        xq, xp, (s0, s1) = _mx_empty(x.shape[0], K, dev), x.data_ptr(), x.stride()
+        if x.get_device() != index:
+            raise ValueError("x is on %s, w on %s" % (x.device, w.device))
+        xp, (s0, s1) = x.data_ptr(), x.stride()
+        codes = scales = None
+        if M > 16:  # up to 16 rows are quantised on their way to the registers
+            scratch = torch.empty(_mx_bytes(M, K), dtype=torch.uint8, device=w.device)
+            codes = scratch.data_ptr()
+            scales = codes + scratch.numel() // 17 * 16
         dtype = dtype or x.dtype
-    if dtype not in _DTYPES:
+    yc = _DTYPES.get(dtype)
+    if yc is None:
         raise ValueError("dtype: %s is none of float32, bfloat16, float16" % dtype)
     bc, bp = 0, None
     if bias is not None:
         bc = _tensor("bias", bias)
-        if tuple(bias.shape) != (N,) or bias.device != dev:
+        if bias.shape != (N,) or bias.get_device() != index:
             raise ValueError("bias: expected [%d] on %s, got %s on %s" % (
-                N, dev, tuple(bias.shape), bias.device))
+                N, w.device, tuple(bias.shape), bias.device))
         bias = bias.contiguous()
         bp = bias.data_ptr()
-    M = xq.shape[0]
-    y = torch.empty((M, N), dtype=dtype, device=dev)
-    _check(lib.ddpg_mx_linear(dev.index, _stream(dev), xc, xp, s0, s1, xq.codes.data_ptr(),
-                              xq.scales.data_ptr(), M, K, w.codes.data_ptr(), w.scales.data_ptr(),
-                              N, bc, bp, _ACTS[act], _DTYPES[dtype], y.data_ptr(), N))
+    y = torch.empty((M, N), dtype=dtype, device=w.device)
+    _check(lib.ddpg_mx_linear(index, _stream(index), xc, xp, s0, s1, codes, scales, M, K, w._codes,
+                              w._scales, N, bc, bp, _ACTS[act], yc, y.data_ptr(), N))
     return y
 
 
@@ -296,21 +288,27 @@ def mx_linear_grad(dy, x, w, need=(True, True), bias=True):
     are the gradients of the matrices that were quantised.  need: whether dx,
     dw are wanted (None otherwise); bias: whether db is."""
     code = _matrix("dy", dy)
-    dev = dy.device
-    _mx("x", x, None, dev)
-    _mx("w", w, x.shape[1], dev)
+    index, dev = dy.get_device(), dy.device
+    _mx("x", x, None, index)
+    _mx("w", w, x.shape[1], index)
     (M, K), N = x.shape, w.shape[0]
-    if tuple(dy.shape) != (M, N):
+    if dy.shape != (M, N):
         raise ValueError("dy: expected [%d, %d], got %s" % (M, N, tuple(dy.shape)))
-    need_dx, need_dw, bias = bool(need[0]), bool(need[1]), bool(bias)
-    dx = torch.empty((M, K), dtype=dy.dtype, device=dev) if need_dx else None
-    dw = torch.empty((N, K), dtype=torch.float32, device=dev) if need_dw else None
-    db = torch.empty(N, dtype=torch.float32, device=dev) if bias else None
-    nb = lib.ddpg_mx_linear_grad_workspace(code, M, N, K, need_dx, need_dw, bias)
+    dx = dw = db = pdx = pdw = pdb = None
+    if need[0]:
+        dx = torch.empty((M, K), dtype=dy.dtype, device=dev)
+        pdx = dx.data_ptr()
+    if need[1]:
+        dw = torch.empty((N, K), dtype=torch.float32, device=dev)
+        pdw = dw.data_ptr()
+    if bias:
+        db = torch.empty(N, dtype=torch.float32, device=dev)
+        pdb = db.data_ptr()
+    nb = lib.ddpg_mx_linear_grad_workspace(code, M, N, K, dx is not None, dw is not None,
+                                           db is not None)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    _check(lib.ddpg_mx_linear_grad(
-        dev.index, _stream(dev), code, dy.data_ptr(), dy.stride(0), dy.stride(1), M, N, K,
-        x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
-        dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dw else None,
-        db.data_ptr() if bias else None, ws.data_ptr(), nb))
+    s0, s1 = dy.stride()
+    _check(lib.ddpg_mx_linear_grad(index, _stream(index), code, dy.data_ptr(), s0, s1, M, N, K,
+                                   x._codes, x._scales, w._codes, w._scales, pdx, pdw, pdb,
+                                   ws.data_ptr(), nb))
     return dx, dw, db

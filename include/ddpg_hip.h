@@ -288,8 +288,8 @@ int ddpg_mx_quantize(int device, void* stream, int dtype, const void* x, int64_t
 int ddpg_mx_dequantize(int device, void* stream, const void* codes, const void* scales,
                        int64_t rows, int64_t cols, int dtype, void* out, int64_t row_stride);
 /* y [M, N] = act(x [M, K] . w [N, K]^T + bias [N]), w quantised.  x != NULL: x is
- * quantised on the way, with x_codes / x_scales (sizes of [M, K]) as scratch;
- * x == NULL: they hold x.  Sums in fp32, one rounding to dtype at the end. */
+ * quantised on the way, with x_codes / x_scales (sizes of [M, K]) as scratch
+ * (unused up to M = 16, NULL will do); x == NULL: they hold x.  Sums in fp32, one rounding to dtype at the end. */
 int ddpg_mx_linear(int device, void* stream, int x_dtype, const void* x, int64_t x_row_stride,
                    int64_t x_col_stride, void* x_codes, void* x_scales, int64_t M, int64_t K,
                    const void* w_codes, const void* w_scales, int64_t N, int bias_dtype,
