@@ -132,8 +132,10 @@ PROTOTYPES = [
     ("ddpg_mx_sizes", _c.c_int, [_i64, _i64, _szp, _szp]),
     ("ddpg_mx_quantize", _c.c_int, [_c.c_int, _P, _c.c_int, _P, _i64, _i64, _i64, _i64, _P, _P]),
     ("ddpg_mx_dequantize", _c.c_int, [_c.c_int, _P, _P, _P, _i64, _i64, _c.c_int, _P, _i64]),
+    ("ddpg_mx_linear_workspace", _c.c_size_t, [_i64, _i64, _i64]),
     ("ddpg_mx_linear", _c.c_int, [_c.c_int, _P, _c.c_int, _P, _i64, _i64, _P, _P, _i64, _i64, _P,
-                                  _P, _i64, _c.c_int, _P, _c.c_int, _c.c_int, _P, _i64]),
+                                  _P, _i64, _c.c_int, _P, _c.c_int, _c.c_int, _P, _i64, _P,
+                                  _c.c_size_t]),
     ("ddpg_mx_linear_grad_workspace", _c.c_size_t, [_c.c_int, _i64, _i64, _i64, _c.c_int,
                                                     _c.c_int, _c.c_int]),
     ("ddpg_mx_linear_grad", _c.c_int, [_c.c_int, _P, _c.c_int, _P, _i64, _i64, _i64, _i64, _i64,

@@ -111,6 +111,8 @@ struct MxPrep {
   MxMat w, x;
   uint8_t *wt, *xt;
   int dy_blocks, w_blocks;
+  unsigned* tickets;  // cleared for the products' joins
+  int ntickets;
 };
 
 // A quantised matrix turned into bfloat16 fragments (mx_gemm.h): rows are its
@@ -199,6 +201,8 @@ __global__ __launch_bounds__(256) void mx_prep_kernel(MxPrep a) {
     float dy[64][65];
   } t;
   const int b = blockIdx.x;
+  if (b == 0)
+    for (int i = threadIdx.x; i < a.ntickets; i += 256) a.tickets[i] = 0;
   if (b < a.dy_blocks)
     mx_dy<DT, mx_planes(DT)>(a, b, t.dy);
   else if (b < a.dy_blocks + a.w_blocks)
@@ -244,32 +248,29 @@ void mx_quantize_launch(hipStream_t st, int dtype, const void* x, int rows, int 
   HIP_TRY(hipGetLastError());
 }
 
-// Which kernel products take: the largest tile that leaves most of the 256 CUs
-// one, and with fewer tiles the kernel that splits the depth over a block's
-// waves.  fp4, us: 16384 x 8192 x 8192 498 on 256 x 256 tiles, 695 on 128 x 128; 1001 x
-// 300 x 400 14.0 on 128 x 128 tiles, 6.7 split.  bf16: 8192 x 4096 x 4096 186 against
-// 250, 1001 x 400 x 3 planes of 300 28.4 against 11.0.
 static bool mx_rows_aligned(const MxOut& o) {
   return o.ldo * elem_size(o.dtype) % 16 == 0 && aligned16(o.y);
 }
 
-enum { MX_BIG, MX_MID, MX_SPLIT, MX_ROWS16 };
+// The kernels of a product: tiles of 256 x 256 and 128 x 128 through LDS, and 64 x 64
+// and 32 x 32 with the depth split over a block's 4 and 8 waves.
+enum { MX_256, MX_128, MX_64, MX_32 };
+static constexpr int kMxTile[] = {256, 128, 64, 32};
+static constexpr int kMxSlab[] = {256 * 256 * 4, 128 * 128 * 4, 64 * 64 * 4, 32 * 32 * 4};
 static long long mx_tiles(int I, int J, int t) {
   return (long long)ceil_div(I, t) * ceil_div(J, t);
-}
-static int mx_pick(long long big, long long mid) {
-  return big >= 200 ? MX_BIG : mid >= 128 ? MX_MID : MX_SPLIT;
 }
 
 template <bool FP4>
 static void mx_gemm_launch(hipStream_t st, MxGemms& p, int pick) {
-  auto launch = [&](auto k, int tile, int threads) {
+  const int tile = kMxTile[pick];
+  auto launch = [&](auto k, int threads) {
     long long n = 0;
     for (int i = 0; i < 2; ++i) {
       MxOut& o = p.g[i].o;
       if (i < p.n) {
         o.vec = mx_rows_aligned(o);
-        n += mx_tiles(o.I, o.J, tile);
+        n += mx_tiles(o.I, o.J, tile) * p.g[i].splits;
       }
       p.end[i] = (int)grid_x(n);
     }
@@ -279,11 +280,10 @@ static void mx_gemm_launch(hipStream_t st, MxGemms& p, int pick) {
     HIP_TRY(hipGetLastError());
   };
   switch (pick) {
-    case MX_BIG: launch(mx_tile_kernel<FP4, 2, 4, 8, 4, 4>, 256, 512); break;
-    case MX_MID: launch(mx_tile_kernel<FP4, 2, 2, 4, 4, 4>, 128, 256); break;
-    case MX_SPLIT: launch(mx_split_kernel<FP4, 4, 4, 4>, 64, 256); break;
-    default:
-      if constexpr (FP4) launch(mx_split_kernel<true, 1, 1, 8>, 16, 512);
+    case MX_256: launch(mx_tile_kernel<FP4, 2, 4, 8, 4, 4>, 512); break;
+    case MX_128: launch(mx_tile_kernel<FP4, 2, 2, 4, 4, 4>, 256); break;
+    case MX_64: launch(mx_split_kernel<FP4, 4, 4, 4, 2>, 256); break;
+    default: launch(mx_split_kernel<FP4, 2, 2, 8, 4>, 512);
   }
 }
 
@@ -292,48 +292,89 @@ static FragOp mx_op(const MxMat& q) {
 }
 
 void mx_linear_launch(hipStream_t st, const MxMat& x, const MxMat& w, const MxOut& o) {
-  MxGemms p{};
   if (!o.I || !o.J) return;
+  MxGemms p{};
   p.n = 1;
-  p.g[0] = {mx_op(x), mx_op(w), x.kt(), 1, o};
-  mx_gemm_launch<true>(st, p, o.I <= 16 ? MX_ROWS16
-                                        : mx_pick(mx_tiles(o.I, o.J, 256), mx_tiles(o.I, o.J, 128)));
+  p.g[0] = {mx_op(x), mx_op(w), x.kt(), 1, o, 1, nullptr, nullptr};
+  // Measured on 60 shapes, us: 256 x 4096 x 1024 5.0 on 32 x 32 tiles, 9.5 on 64; 512 x
+  // 4096 x 4096 13.1 on 64 x 64, 20.2 on 32, 19.5 on 128; 4096 x 1024 x 1024 11.3 on 128 x
+  // 128, 14.7 on 64, 17.1 on 256; 8192 x 2048 x 2048 26.5 on 256 x 256, 32.8 on 128
+  auto tiles = [&](int pick) { return mx_tiles(o.I, o.J, kMxTile[pick]); };
+  mx_gemm_launch<true>(st, p, tiles(MX_256) >= 256  ? MX_256
+                              : tiles(MX_32) <= 384 ? MX_32
+                              : tiles(MX_64) <= 512 ? MX_64
+                                                    : MX_128);
 }
 
-// at most 16 rows, quantised on the way
+// Whether the rows of x are quantised by every block of 16 columns of the
+// product.  A row of 8192 values: 7.5 us so, 9.5 in two launches; 16 rows of 2048 6.5
+// and 7.1, of 4096 10.2 and 7.8; 64 of 512 7.6 and 6.8 (and the launch's host time).
+static bool mx_rows_ok(int64_t M, int64_t K) { return M <= 64 && M * K <= 32768; }
 void mx_linear_rows_launch(hipStream_t st, int dtype, const void* x, long long sr, long long sc,
                            int M, int K, const MxMat& w, MxOut o) {
   if (!M || !o.J) return;
   o.vec = mx_rows_aligned(o);
-  const RawX r{x, sr, sc, M, K, dtype, sc == 1};
+  const RawX r{x, sr, sc, M, K, sc == 1};
   by_dtype(dtype, [&](auto dt) {
-    hipLaunchKernelGGL((mx_rows_kernel<decltype(dt)::value, 8>), dim3(ceil_div(o.J, 16)), dim3(512),
-                       0, st, r, mx_op(w), w.kt(), o);
+    constexpr int DT = decltype(dt)::value;
+    auto k = M <= 16   ? mx_rows_kernel<DT, 1, 8>
+             : M <= 32 ? mx_rows_kernel<DT, 2, 8>
+                       : mx_rows_kernel<DT, 4, 8>;
+    hipLaunchKernelGGL(k, dim3(ceil_div(o.J, 16)), dim3(512), 0, st, r, mx_op(w), w.kt(), o);
   });
   HIP_TRY(hipGetLastError());
 }
 
-// The gradient's workspace, in order.
-struct MxGradWs {
-  size_t flat, wt, turned, xt, part, total;
+// The gradient's plan: the kernel, the depth's splits and the workspace, in
+// order.  Kernel and splits go by both products, so that a result does not depend
+// on which are asked for.
+struct MxGradPlan {
+  size_t flat, wt, turned, xt, part, tickets, slab[2], total;  // slab: of dX, dW
   int sn, sm, P;  // depth steps over N, over M
+  int pick, splits[2];
+  int ntickets;
 };
-static MxGradWs mx_grad_ws(int dtype, int M, int N, int K, bool dx, bool dw, bool db) {
-  MxGradWs w{};
+static MxGradPlan mx_grad_plan(int dtype, int M, int N, int K, bool dx, bool dw, bool db) {
+  MxGradPlan w{};
   w.P = mx_planes(dtype);
   w.sn = ceil_div(N, 64) * 2;
   w.sm = ceil_div(M, 64) * 2;
-  auto frags = [](int rows, size_t steps) { return (size_t)ceil_div(rows, 64) * 4 * steps * 1024; };
+  const long long steps[2] = {(long long)w.P * w.sn, (long long)w.P * w.sm};
+  const int I[2] = {M, N};
+  auto tiles = [&](int q, int pick) { return mx_tiles(I[q], K, kMxTile[pick]); };
+  auto all = [&](int pick) { return tiles(0, pick) * steps[0] + tiles(1, pick) * steps[1]; };
+  // Each kernel up to the work (a tile costs about 16 depth steps besides its own)
+  // it is best at; us, bf16: 1362 x 195 x 2659 26.3 on 64 x 64 tiles, 26.5 on 32, 37.9 on 128;
+  // 2048 x 2048 x 2048 57.8 on 128 x 128, 71.1 on 64, 72.6 on 256; 4096 x 2048 x 2048 95.4 on 256
+  // x 256, 106.7 on 128
+  auto cost = [&](int pick) { return all(pick) + 16 * (tiles(0, pick) + tiles(1, pick)); };
+  w.pick = cost(MX_256) >= 16000    ? MX_256
+           : cost(MX_32) <= 40000   ? MX_32
+           : cost(MX_64) <= 160000  ? MX_64
+                                    : MX_128;
+  // a block's depth: an equal share of a launch that fills the chip, but no less
+  // than what makes the join worth it
+  const long long least[] = {32, 24, 32, 64}, fill[] = {256, 256, 512, 512};
+  const long long share = std::max(least[w.pick], (all(w.pick) + fill[w.pick] - 1) / fill[w.pick]);
   size_t off = 0;
   auto place = [&](size_t& at, bool need, size_t bytes) {
     at = off;
     if (need) off += (bytes + 255) / 256 * 256;
   };
+  auto frags = [](int rows, size_t steps) { return (size_t)ceil_div(rows, 64) * 4 * steps * 1024; };
   place(w.flat, dx, frags(M, (size_t)w.P * w.sn));
   place(w.wt, dx, frags(K, w.sn));
   place(w.turned, dw, frags(N, (size_t)w.P * w.sm));
   place(w.xt, dw, frags(K, w.sm));
   place(w.part, db, (size_t)ceil_div(M, 64) * N * 4);
+  for (int q = 0; q < 2; ++q) {
+    w.splits[q] = (int)std::min<long long>(32, std::max<long long>(1, (steps[q] + share / 2) / share));
+    if (w.splits[q] > 1) w.ntickets += (int)tiles(q, w.pick);
+  }
+  place(w.tickets, w.ntickets, (size_t)w.ntickets * 4);
+  for (int q = 0; q < 2; ++q)
+    place(w.slab[q], w.splits[q] > 1 && (q ? dw : dx),
+          (size_t)tiles(q, w.pick) * w.splits[q] * kMxSlab[w.pick]);
   w.total = off;
   return w;
 }
@@ -342,7 +383,7 @@ void mx_linear_grad_launch(hipStream_t st, int dtype, const void* dy, long long 
                            const MxMat& x, const MxMat& w, void* dx, float* dw, float* db,
                            uint8_t* ws) {
   const int M = x.rows, N = w.rows, K = x.cols;
-  const MxGradWs L = mx_grad_ws(dtype, M, N, K, dx, dw, db);
+  const MxGradPlan L = mx_grad_plan(dtype, M, N, K, dx, dw, db);
   MxPrep a{};
   a.dy = dy;
   a.sr = sr;
@@ -361,6 +402,8 @@ void mx_linear_grad_launch(hipStream_t st, int dtype, const void* dy, long long 
                   nx = dw ? m64 * kt : 0;
   a.dy_blocks = (int)grid_x(nd);
   a.w_blocks = (int)grid_x(nw);
+  a.tickets = reinterpret_cast<unsigned*>(ws + L.tickets);
+  a.ntickets = L.ntickets;
   if (nd + nw + nx)
     by_dtype(dtype, [&](auto dt) {
       hipLaunchKernelGGL(mx_prep_kernel<decltype(dt)::value>, dim3(grid_x(nd + nw + nx)), dim3(256),
@@ -368,26 +411,30 @@ void mx_linear_grad_launch(hipStream_t st, int dtype, const void* dy, long long 
     });
   HIP_TRY(hipGetLastError());
   MxGemms p{};
-  auto add = [&](const uint8_t* I, const uint8_t* J, int ni, int nj, int steps, void* C, int type) {
-    if (!ni || !nj) return;
+  unsigned* tickets = reinterpret_cast<unsigned*>(ws + L.tickets);
+  auto add = [&](int q, const uint8_t* I, const uint8_t* J, int ni, int steps, void* C, int type) {
+    if (!ni || !K) return;
+    // dX's tickets first, then dW's
+    unsigned* t = tickets + (q && L.splits[0] > 1 ? mx_tiles(M, K, kMxTile[L.pick]) : 0);
     p.g[p.n++] = {{I, nullptr, ceil_div(ni, 64) * 4},
-                  {J, nullptr, ceil_div(nj, 64) * 4},
+                  {J, nullptr, ceil_div(K, 64) * 4},
                   steps,
                   L.P,
-                  {C, nullptr, nj, ni, nj, type, 0, DDPG_ACT_NONE, 0}};
+                  {C, nullptr, K, ni, K, type, 0, DDPG_ACT_NONE, 0},
+                  L.splits[q],
+                  reinterpret_cast<float*>(ws + L.slab[q]),
+                  t};
   };
-  // the deeper product's tiles first: the shorter ones fill in behind them
+  // the deeper product's blocks first: the shorter ones fill in behind them
   const bool dw_first = L.sm > L.sn;
-  if (dw && dw_first) add(a.turned, a.xt, N, K, L.sm, dw, T_FP32);
-  if (dx) add(a.flat, a.wt, M, K, L.sn, dx, dtype);
-  if (dw && !dw_first) add(a.turned, a.xt, N, K, L.sm, dw, T_FP32);
+  if (dw && dw_first) add(1, a.turned, a.xt, N, L.sm, dw, T_FP32);
+  if (dx) add(0, a.flat, a.wt, M, L.sn, dx, dtype);
+  if (dw && !dw_first) add(1, a.turned, a.xt, N, L.sm, dw, T_FP32);
   p.db = db;
   p.db_part = a.part;
   p.db_n = db ? N : 0;
   p.db_parts = (int)m64;
-  // by both products' tiles, so that a result does not depend on which are asked
-  mx_gemm_launch<false>(st, p, mx_pick(mx_tiles(M, K, 256) + mx_tiles(N, K, 256),
-                                       mx_tiles(M, K, 128) + mx_tiles(N, K, 128)));
+  mx_gemm_launch<false>(st, p, L.pick);
 }
 
 }  // namespace ddpg
@@ -435,18 +482,32 @@ int ddpg_mx_dequantize(int device, void* stream, const void* codes, const void* 
   });
 }
 
+size_t ddpg_mx_linear_workspace(int64_t M, int64_t K, int64_t N) {
+  if (M < 0 || K < 0 || N < 0 || M > kMxMaxDim || K > kMxMaxDim || N > kMxMaxDim) return 0;
+  return mx_rows_ok(M, K) ? 0 : mx_code_bytes(M, K) + mx_scale_bytes(M, K);
+}
+
 int ddpg_mx_linear(int device, void* stream, int x_dtype, const void* x, int64_t x_row_stride,
-                   int64_t x_col_stride, void* x_codes, void* x_scales, int64_t M, int64_t K,
-                   const void* w_codes, const void* w_scales, int64_t N, int bias_dtype,
-                   const void* bias, int act, int dtype, void* y, int64_t y_row_stride) {
+                   int64_t x_col_stride, const void* x_codes, const void* x_scales, int64_t M,
+                   int64_t K, const void* w_codes, const void* w_scales, int64_t N, int bias_dtype,
+                   const void* bias, int act, int dtype, void* y, int64_t y_row_stride, void* ws,
+                   size_t ws_bytes) {
   return guard(nullptr, [&] {
-    const bool rows = x && M <= 16;  // needs no scratch
-    const MxMat xq = mx_mat("mx_linear x", x_codes, x_scales, M, rows ? 0 : K);
+    mx_check_dims("mx_linear x", M, K);
     const MxMat wq = mx_mat("mx_linear w", w_codes, w_scales, N, K);
+    MxMat xq{nullptr, nullptr, (int)M, (int)K};
     check_dtype("mx_linear", dtype);
-    if (x) check_dtype("mx_linear x", x_dtype);
     if (bias) check_dtype("mx_linear bias", bias_dtype);
     if (act < DDPG_ACT_NONE || act > DDPG_ACT_TANH) throw einval("mx_linear: act %d", act);
+    const bool rows = x && mx_rows_ok(M, K);
+    if (!x) {
+      xq = mx_mat("mx_linear x", x_codes, x_scales, M, K);
+    } else {
+      check_dtype("mx_linear x", x_dtype);
+      const size_t need = rows ? 0 : mx_code_bytes(M, K) + mx_scale_bytes(M, K);
+      if (ws_bytes < need || (need && !ws) || (need && !aligned16(ws)))
+        throw einval("mx_linear: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    }
     if (!M || !N) return;
     if (!y) throw einval("mx_linear: null output");
     if (y_row_stride < N) throw einval("mx_linear: rows %lld apart overlap", (long long)y_row_stride);
@@ -457,9 +518,13 @@ int ddpg_mx_linear(int device, void* stream, int x_dtype, const void* x, int64_t
       mx_linear_rows_launch(st, x_dtype, x, x_row_stride, x_col_stride, (int)M, (int)K, wq, o);
       return;
     }
-    if (x)
-      mx_quantize_launch(st, x_dtype, x, (int)M, (int)K, x_row_stride, x_col_stride,
-                         static_cast<uint8_t*>(x_codes), static_cast<uint8_t*>(x_scales));
+    if (x) {
+      uint8_t* codes = static_cast<uint8_t*>(ws);
+      uint8_t* scales = codes + mx_code_bytes(M, K);
+      mx_quantize_launch(st, x_dtype, x, (int)M, (int)K, x_row_stride, x_col_stride, codes, scales);
+      xq.codes = codes;
+      xq.scales = scales;
+    }
     mx_linear_launch(st, xq, wq, o);
   });
 }
@@ -467,7 +532,7 @@ int ddpg_mx_linear(int device, void* stream, int x_dtype, const void* x, int64_t
 size_t ddpg_mx_linear_grad_workspace(int dtype, int64_t M, int64_t N, int64_t K, int dx, int dw,
                                      int db) {
   if (M < 0 || N < 0 || K < 0 || M > kMxMaxDim || N > kMxMaxDim || K > kMxMaxDim) return 0;
-  return mx_grad_ws(dtype, (int)M, (int)N, (int)K, dx != 0, dw != 0, db != 0).total;
+  return mx_grad_plan(dtype, (int)M, (int)N, (int)K, dx != 0, dw != 0, db != 0).total;
 }
 
 int ddpg_mx_linear_grad(int device, void* stream, int dtype, const void* dy, int64_t dy_row_stride,
@@ -483,7 +548,7 @@ int ddpg_mx_linear_grad(int device, void* stream, int dtype, const void* dy, int
                             N, dx ? K : 0);
     mx_check_dims("mx_linear_grad", M, K);
     if (M && N && !dy) throw einval("mx_linear_grad: null dy");
-    const size_t need = mx_grad_ws(dtype, (int)M, (int)N, (int)K, dx, dw, db).total;
+    const size_t need = mx_grad_plan(dtype, (int)M, (int)N, (int)K, dx, dw, db).total;
     if (ws_bytes < need || (need && !ws) || !aligned16(ws))
       throw einval("mx_linear_grad: workspace of %zu bytes, %zu needed", ws_bytes, need);
     OnDevice on(device);

@@ -35,6 +35,10 @@ struct MxGemm {
   int kt;      // depth steps of J
   int planes;  // I holds `planes` times kt steps a row group; J's repeat
   MxOut o;
+  // the depth in `splits` blocks a tile, joined in the launch (mx_join)
+  int splits;
+  float* slab;        // [tile][split][a block's sums]
+  unsigned* tickets;  // [tile], zero before and after the launch
 };
 
 // One launch: n products (blocks 0 .. end[0] - 1, .. end[1] - 1), then 64 columns
@@ -172,6 +176,65 @@ DDPG_DEV void tile_of(int lin, int ni, int nj, int& ti, int& tj) {
   tj = in / rows;
 }
 
+// Which of a product's blocks this is: tile, split and its depth steps.
+struct MxPart {
+  int ti, tj, tile, split, k0, n;
+};
+DDPG_DEV MxPart mx_part(const MxGemm& g, int lin, int bi, int bj) {
+  const int ni = (g.o.I + bi - 1) / bi, nj = (g.o.J + bj - 1) / bj, nt = ni * nj;
+  MxPart p;
+  p.split = lin / nt;
+  tile_of(lin - p.split * nt, ni, nj, p.ti, p.tj);
+  p.tile = p.ti * nj + p.tj;
+  const long long nk = (long long)g.kt * g.planes;
+  p.k0 = (int)(nk * p.split / g.splits);
+  p.n = (int)(nk * (p.split + 1) / g.splits) - p.k0;
+  return p;
+}
+
+// The blocks of a tile store their sums (lane after lane, 16 bytes each) past the
+// XCDs' separate L2s (sc1), wait for the stores, and one thread takes a ticket;
+// the block with the last ticket adds the splits' sums in split order, so the
+// result does not depend on which came last, and puts the ticket back to zero.
+// True in that block.  NF f32x4 a thread; threads `on` take part.
+template <int NF>
+DDPG_DEV bool mx_join(const MxGemm& g, const MxPart& p, f32x4* acc, int thread, int threads,
+                      bool on) {
+  __shared__ unsigned last;
+  const unsigned bytes = (unsigned)(NF * threads * 16);  // a block's sums
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(reinterpret_cast<char*>(g.slab) + (size_t)p.tile * g.splits * bytes), 0, 0x7fffffff,
+      0x00020000);
+  if (on)
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[f]), rs,
+                                             p.split * bytes + (f * threads + thread) * 16, 0,
+                                             KC_SC1);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have left
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const unsigned was =
+        __hip_atomic_fetch_add(g.tickets + p.tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = was == (unsigned)(g.splits - 1);
+    if (last)
+      __hip_atomic_store(g.tickets + p.tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last) return false;
+  if (on) {
+#pragma unroll
+    for (int f = 0; f < NF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < g.splits; ++s)
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+        acc[f] += __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                       rs, s * bytes + (f * threads + thread) * 16, 0, KC_SC1));
+  }
+  return true;
+}
+
 // ---------------------------------------------------------------- LDS tiles
 template <int OFF>
 DDPG_DEV u32x4 lds_b128(unsigned a) {
@@ -234,11 +297,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ, wj = wave % WJ;
-  const int ni = (g.o.I + C::GI * 16 - 1) / (C::GI * 16);
-  const int nj = (g.o.J + C::GJ * 16 - 1) / (C::GJ * 16);
-  int ti, tj;
-  tile_of(blockIdx.x - (second ? p.end[0] : 0), ni, nj, ti, tj);
-  const int nk = g.kt * g.planes;
+  const MxPart pt = mx_part(g, blockIdx.x - (second ? p.end[0] : 0), C::GI * 16, C::GJ * 16);
+  const int ti = pt.ti, tj = pt.tj, nk = pt.n;
+  int jk = pt.k0 % max(g.kt, 1);  // J's depth step of the next load (I's planes go on, J's repeat)
 
   // this wave's pieces of a step: source of the next step to load, LDS place.
   // Row groups past the operand's last are read from the last one's place
@@ -252,7 +313,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
     isj[p] = f >= C::GI;
     const int grp = isj[p] ? min(tj * C::GJ + f - C::GI, g.J.groups - 1)
                            : min(ti * C::GI + f, g.I.groups - 1);
-    src[p] = (isj[p] ? g.J.p + (size_t)grp * g.kt * 1024 : g.I.p + (size_t)grp * nk * 1024) +
+    src[p] = (isj[p] ? g.J.p + ((size_t)grp * g.kt + jk) * 1024
+                     : g.I.p + ((size_t)grp * g.kt * g.planes + pt.k0) * 1024) +
              lane * 16;
   }
 #pragma unroll
@@ -261,9 +323,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
     const bool j = f >= C::GI / 4;
     const int grp = j ? min(tj * (C::GJ / 4) + f - C::GI / 4, g.J.groups / 4 - 1)
                       : min(ti * (C::GI / 4) + f, g.I.groups / 4 - 1);
-    ssrc[p] = (j ? g.J.scales : g.I.scales) + (size_t)grp * g.kt * 256 + lane * 4;
+    ssrc[p] = (j ? g.J.scales : g.I.scales) + ((size_t)grp * g.kt + pt.k0) * 256 + lane * 4;
   }
-  int jk = 0;  // J's depth step of the next load (I's planes go on, J's repeat)
   lds_char* const base = (lds_char*)smem;
   auto load_piece = [&](int slot, auto p_c) {
     constexpr int p = decltype(p_c)::value;
@@ -388,6 +449,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
       if (s + 1 < nk) step(s + 1, S1{}, std::true_type{});
     }
   }
+  if (!FP4 && g.splits > 1 && !mx_join<TI * TJ>(g, pt, &acc[0][0], threadIdx.x, C::NT, true))
+    return;
   __syncthreads();  // the ring is done with: it carries the results out
   float bias[TJ][4];
 #pragma unroll
@@ -401,16 +464,109 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
 }
 
 // ---------------------------------------------------------------- few tiles
-// One block: TI x TJ fragments of C, its NW waves taking every NW-th depth step
-// with operands straight from memory, two steps ahead; the waves' sums are
-// joined in LDS in wave order.
-// Up to 16 rows of x as they are: the block's products quantise them on their way
-// to the registers (each block again: x is small and stays in the caches, and a
-// launch is saved).
+// One block: TI x TJ fragments of C, its NW waves taking every NW-th of the
+// block's depth steps with operands straight from memory, PF steps ahead; the
+// waves' sums are joined in LDS in wave order.
+template <bool FP4, int TI, int TJ, int NW, int PF>
+__global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemms p) {
+  __shared__ f32x4 part[NW][TI * TJ][64];
+  static_assert(TI * TJ < NW || TI * TJ % NW == 0, "whole fragments a wave");
+  if ((int)blockIdx.x >= p.end[1]) {
+    mx_db<NW>(p, blockIdx.x - p.end[1], *reinterpret_cast<double(*)[NW][64]>(part));
+    return;
+  }
+  const bool second = (int)blockIdx.x >= p.end[0];
+  const MxGemm& g = p.g[second];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const MxPart pt = mx_part(g, blockIdx.x - (second ? p.end[0] : 0), TI * 16, TJ * 16);
+  const int nk = pt.n;
+  f32x4 acc[TI][TJ];
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // the fragments' scales are adjacent bytes of one dword (TI, TJ: 1, 2 or 4)
+  const int gi = pt.ti * TI, gj = pt.tj * TJ;
+  const uint8_t *pi[TI], *pj[TJ];
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+    pi[i] = g.I.p + ((size_t)min(gi + i, g.I.groups - 1) * g.kt * g.planes + pt.k0) * 1024 + lane * 16;
+#pragma unroll
+  for (int j = 0; j < TJ; ++j)
+    pj[j] = g.J.p + (size_t)min(gj + j, g.J.groups - 1) * g.kt * 1024 + lane * 16;
+  const uint8_t* qi = FP4 ? g.I.scales + (size_t)(gi >> 2) * g.kt * 256 + lane * 4 : nullptr;
+  const uint8_t* qj = FP4 ? g.J.scales + (size_t)(gj >> 2) * g.kt * 256 + lane * 4 : nullptr;
+  struct Step {
+    u32x4 i[TI], j[TJ];
+    unsigned si, sj;
+  };
+  auto load = [&](int s, Step& f) {
+    const int k = FP4 ? s : (s + pt.k0) % g.kt;
+#pragma unroll
+    for (int i = 0; i < TI; ++i) f.i[i] = *reinterpret_cast<const u32x4*>(pi[i] + (size_t)s * 1024);
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) f.j[j] = *reinterpret_cast<const u32x4*>(pj[j] + (size_t)k * 1024);
+    f.si = f.sj = 0;
+    if constexpr (FP4) {
+      f.si = *reinterpret_cast<const unsigned*>(qi + (size_t)k * 256) >> (8 * (gi & 3));
+      f.sj = *reinterpret_cast<const unsigned*>(qj + (size_t)k * 256) >> (8 * (gj & 3));
+    }
+  };
+  {
+    Step f[PF];
+    static_for<PF>([&](auto u) {
+      constexpr int U = decltype(u)::value;
+      if (wave + U * NW < nk) load(wave + U * NW, f[U]);
+    });
+    for (int s = wave; s < nk; s += PF * NW)
+      static_for<PF>([&](auto u) {
+        constexpr int U = decltype(u)::value;
+        if (s + U * NW < nk) {
+          static_for<TI * TJ>([&](auto q_c) {
+            constexpr int i = decltype(q_c)::value / TJ, j = decltype(q_c)::value % TJ;
+            acc[i][j] = frag_mfma<FP4, j, i>(f[U].j[j], f[U].i[i], acc[i][j], f[U].sj, f[U].si);
+          });
+          if (s + (U + PF) * NW < nk) load(s + (U + PF) * NW, f[U]);
+        }
+      });
+  }
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) part[wave][i * TJ + j][lane] = acc[i][j];
+  __syncthreads();
+  // fragments wave, wave + NW ..: at most NF a wave
+  constexpr int NF = (TI * TJ + NW - 1) / NW;
+  f32x4 sum[NF];
+  const bool on = wave < TI * TJ;
+#pragma unroll
+  for (int q = 0; q < NF; ++q) {
+    const int f = min(wave + q * NW, TI * TJ - 1);
+    sum[q] = part[0][f][lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) sum[q] += part[w][f][lane];
+  }
+  constexpr int ON = TI * TJ < NW ? TI * TJ : NW;  // waves with a fragment
+  if (!FP4 && g.splits > 1 && !mx_join<NF>(g, pt, sum, threadIdx.x, ON * 64, on)) return;
+  if (!on) return;
+#pragma unroll
+  for (int q = 0; q < NF; ++q) {
+    const int f = wave + q * NW, i = f / TJ, j = f % TJ;
+    const int jj = (gj + j) * 16 + (lane >> 4) * 4;
+    float b[4];
+    mx_bias(g.o, jj, b);
+    mx_store(g.o, (gi + i) * 16 + (lane & 15), jj, sum[q], b);
+  }
+}
+
+// Rows of x as they are: the block's products quantise them on their way to the
+// registers (each block again: x is small and stays in the caches, and a launch
+// is saved).
 struct RawX {
   const void* p;
   long long sr, sc;
-  int rows, cols, dtype;
+  int rows, cols;
   int vec;  // columns adjacent
 };
 
@@ -430,120 +586,60 @@ DDPG_DEV void mx_load_block(const typename Elem<DT>::type* p, long long sc, bool
   }
 }
 
-// y = act(x w^T + b) for at most 16 rows: a block makes 16 columns, its waves
+// y = act(x w^T + b) for at most 16 TI rows: a block makes 16 columns, its waves
 // taking every NW-th depth step, the sums joined in wave order.
-template <int DT, int NW>
+template <int DT, int TI, int NW>
 __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(RawX x, FragOp w, int kt, MxOut o) {
-  __shared__ f32x4 part[NW][64];
+  __shared__ f32x4 part[NW][TI][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, gj = blockIdx.x;
-  const typename Elem<DT>::type* xp =
-      static_cast<const typename Elem<DT>::type*>(x.p) + min(lane & 15, x.rows - 1) * x.sr;
+  typedef typename Elem<DT>::type T;
+  // rows past x's repeat its last one, their results are not stored
+  const T* xp[TI];
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+    xp[i] = static_cast<const T*>(x.p) + min(i * 16 + (lane & 15), x.rows - 1) * x.sr;
   const uint8_t* pj = w.p + (size_t)gj * kt * 1024 + lane * 16;
   const uint8_t* qj = w.scales + (size_t)(gj >> 2) * kt * 256 + lane * 4 + (gj & 3);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int s = wave; s < kt; s += NW) {
-    const u32x4 j = *reinterpret_cast<const u32x4*>(pj + (size_t)s * 1024);
-    const unsigned sj = qj[(size_t)s * 256];
-    // rows past x's repeat its last one, their results are not stored
-    float v[32];
-    mx_load_block<DT>(xp, x.sc, x.vec, s * 128 + (lane >> 4) * 32, x.cols, v);
-    unsigned si;
-    const u32x4 i = mx_quantize_block(v, si);
-    acc = mx_mfma<0, 0>(j, i, acc, sj, si);
+  f32x4 acc[TI];
+#pragma unroll
+  for (int i = 0; i < TI; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // U steps at a time, so that their loads overlap (the last may repeat a step,
+  // whose product is left out)
+  constexpr int U = TI == 1 ? 2 : 1;
+  for (int s0 = wave; s0 < kt; s0 += U * NW) {
+    u32x4 j[U];
+    unsigned sj[U];
+    float v[U][TI][32];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = min(s0 + u * NW, kt - 1);
+      j[u] = *reinterpret_cast<const u32x4*>(pj + (size_t)s * 1024);
+      sj[u] = qj[(size_t)s * 256];
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+        mx_load_block<DT>(xp[i], x.sc, x.vec, s * 128 + (lane >> 4) * 32, x.cols, v[u][i]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + u * NW < kt)
+#pragma unroll
+        for (int i = 0; i < TI; ++i) {
+          unsigned si;
+          const u32x4 q = mx_quantize_block(v[u][i], si);
+          acc[i] = mx_mfma<0, 0>(j[u], q, acc[i], sj[u], si);
+        }
   }
-  part[wave][lane] = acc;
+#pragma unroll
+  for (int i = 0; i < TI; ++i) part[wave][i][lane] = acc[i];
   __syncthreads();
-  if (wave) return;
-  for (int s = 1; s < NW; ++s) acc += part[s][lane];
+  if (wave >= TI) return;
+  f32x4 sum = part[0][wave][lane];
+#pragma unroll
+  for (int s = 1; s < NW; ++s) sum += part[s][wave][lane];
   const int jj = gj * 16 + (lane >> 4) * 4;
   float b[4];
   mx_bias(o, jj, b);
-  mx_store(o, lane & 15, jj, acc, b);
-}
-
-template <bool FP4, int TI, int TJ, int NW>
-__global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemms p) {
-  __shared__ f32x4 part[NW][TI * TJ][64];
-  if ((int)blockIdx.x >= p.end[1]) {
-    mx_db<NW>(p, blockIdx.x - p.end[1], *reinterpret_cast<double(*)[NW][64]>(part));
-    return;
-  }
-  const bool second = (int)blockIdx.x >= p.end[0];
-  const MxGemm& g = p.g[second];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int ni = (g.o.I + TI * 16 - 1) / (TI * 16), nj = (g.o.J + TJ * 16 - 1) / (TJ * 16);
-  int ti, tj;
-  tile_of(blockIdx.x - (second ? p.end[0] : 0), ni, nj, ti, tj);
-  const int nk = g.kt * g.planes;
-  f32x4 acc[TI][TJ];
-#pragma unroll
-  for (int i = 0; i < TI; ++i)
-#pragma unroll
-    for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const uint8_t *pi[TI], *pj[TJ];
-#pragma unroll
-  for (int i = 0; i < TI; ++i)
-    pi[i] = g.I.p + (size_t)min(ti * TI + i, g.I.groups - 1) * nk * 1024 + lane * 16;
-#pragma unroll
-  for (int j = 0; j < TJ; ++j)
-    pj[j] = g.J.p + (size_t)min(tj * TJ + j, g.J.groups - 1) * g.kt * 1024 + lane * 16;
-  // the scale dwords of the 64-row groups the fragments lie in (TI, TJ: 1 or 4)
-  const int gi = ti * TI, gj = tj * TJ;
-  const uint8_t* qi = FP4 ? g.I.scales + (size_t)min(gi >> 2, g.I.groups / 4 - 1) * g.kt * 256 + lane * 4 : nullptr;
-  const uint8_t* qj = FP4 ? g.J.scales + (size_t)min(gj >> 2, g.J.groups / 4 - 1) * g.kt * 256 + lane * 4 : nullptr;
-  struct Step {
-    u32x4 i[TI], j[TJ];
-    unsigned si, sj;
-  };
-  auto load = [&](int s, Step& f) {
-    const int k = FP4 ? s : s % g.kt;
-#pragma unroll
-    for (int i = 0; i < TI; ++i) f.i[i] = *reinterpret_cast<const u32x4*>(pi[i] + (size_t)s * 1024);
-#pragma unroll
-    for (int j = 0; j < TJ; ++j) f.j[j] = *reinterpret_cast<const u32x4*>(pj[j] + (size_t)k * 1024);
-    f.si = f.sj = 0;
-    if constexpr (FP4) {
-      f.si = *reinterpret_cast<const unsigned*>(qi + (size_t)k * 256);
-      f.sj = *reinterpret_cast<const unsigned*>(qj + (size_t)k * 256);
-      if (TI == 1) f.si >>= 8 * (gi & 3);
-      if (TJ == 1) f.sj >>= 8 * (gj & 3);
-    }
-  };
-  auto mul = [&](const Step& f) {
-    static_for<TI * TJ>([&](auto q_c) {
-      constexpr int i = decltype(q_c)::value / TJ, j = decltype(q_c)::value % TJ;
-      acc[i][j] = frag_mfma<FP4, j, i>(f.j[j], f.i[i], acc[i][j], f.sj, f.si);
-    });
-  };
-  {
-    Step a, b;
-    int s = wave;
-    if (s < nk) load(s, a);
-    if (s + NW < nk) load(s + NW, b);
-    for (; s < nk; s += 2 * NW) {
-      mul(a);
-      if (s + 2 * NW < nk) load(s + 2 * NW, a);
-      if (s + NW < nk) {
-        mul(b);
-        if (s + 3 * NW < nk) load(s + 3 * NW, b);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < TI; ++i)
-#pragma unroll
-    for (int j = 0; j < TJ; ++j) part[wave][i * TJ + j][lane] = acc[i][j];
-  __syncthreads();
-  for (int f = wave; f < TI * TJ; f += NW) {
-    f32x4 s = part[0][f][lane];
-    for (int w = 1; w < NW; ++w) s += part[w][f][lane];
-    const int i = f / TJ, j = f % TJ;
-    const int jj = (tj * TJ + j) * 16 + (lane >> 4) * 4;
-    float b[4];
-    mx_bias(g.o, jj, b);
-    mx_store(g.o, (ti * TI + i) * 16 + (lane & 15), jj, s, b);
-  }
+  mx_store(o, wave * 16 + (lane & 15), jj, sum, b);
 }
 
 }  // namespace ddpg

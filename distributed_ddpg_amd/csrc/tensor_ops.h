@@ -37,6 +37,19 @@ struct __attribute__((packed, aligned(2))) U16B {
   uint32_t v[4];
 };
 
+// ... past the caches if NT: for bytes that are used once
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+template <bool NT>
+DDPG_DEV U16B load16(const void* p) {
+  const u32x4_any* q = static_cast<const u32x4_any*>(p);
+  const u32x4_any v = NT ? __builtin_nontemporal_load(q) : *q;
+  return {{v[0], v[1], v[2], v[3]}};
+}
+DDPG_DEV void store16_nt(void* p, const U16B& u) {
+  const u32x4_any v = {u.v[0], u.v[1], u.v[2], u.v[3]};
+  __builtin_nontemporal_store(v, static_cast<u32x4_any*>(p));
+}
+
 // An element type: its loads widened to fp32 (exact), its stores one rounding
 // to nearest even; the 16 / sizeof elements of U16B likewise.
 template <int DT>

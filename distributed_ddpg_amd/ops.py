@@ -243,6 +243,7 @@ def mx_linear(x, w, bias=None, act=None, dtype=None):
     MXTensor)."""
     _mx("w", w)
     (N, K), index = w.shape, w._index
+    wp, nb = None, 0
     if act not in _ACTS:
         raise ValueError("act: %r is none of None, 'elu', 'tanh'" % (act,))
     if isinstance(x, MXTensor):
@@ -258,10 +259,10 @@ def mx_linear(x, w, bias=None, act=None, dtype=None):
             raise ValueError("x is on %s, w on %s" % (x.device, w.device))
         xp, (s0, s1) = x.data_ptr(), x.stride()
         codes = scales = None
-        if M > 16:  # up to 16 rows are quantised on their way to the registers
-            scratch = torch.empty(_mx_bytes(M, K), dtype=torch.uint8, device=w.device)
-            codes = scratch.data_ptr()
-            scales = codes + scratch.numel() // 17 * 16
+        nb = lib.ddpg_mx_linear_workspace(M, K, N)
+        if nb:
+            ws = torch.empty(nb, dtype=torch.uint8, device=w.device)
+            wp = ws.data_ptr()
         dtype = dtype or x.dtype
     yc = _DTYPES.get(dtype)
     if yc is None:
@@ -276,7 +277,8 @@ def mx_linear(x, w, bias=None, act=None, dtype=None):
         bp = bias.data_ptr()
     y = torch.empty((M, N), dtype=dtype, device=w.device)
     _check(lib.ddpg_mx_linear(index, _stream(index), xc, xp, s0, s1, codes, scales, M, K, w._codes,
-                              w._scales, N, bc, bp, _ACTS[act], yc, y.data_ptr(), N))
+                              w._scales, N, bc, bp, _ACTS[act], yc, y.data_ptr(), N, wp,
+                              nb))
     return y
 
 

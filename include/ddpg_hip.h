@@ -288,12 +288,15 @@ int ddpg_mx_quantize(int device, void* stream, int dtype, const void* x, int64_t
 int ddpg_mx_dequantize(int device, void* stream, const void* codes, const void* scales,
                        int64_t rows, int64_t cols, int dtype, void* out, int64_t row_stride);
 /* y [M, N] = act(x [M, K] . w [N, K]^T + bias [N]), w quantised.  x != NULL: x is
- * quantised on the way, with x_codes / x_scales (sizes of [M, K]) as scratch
- * (unused up to M = 16, NULL will do); x == NULL: they hold x.  Sums in fp32, one rounding to dtype at the end. */
+ * quantised on the way, in ws (ddpg_mx_linear_workspace bytes, 16-byte aligned; 0
+ * where a few rows are quantised inside the product); x == NULL: x_codes /
+ * x_scales hold it.  Sums in fp32, one rounding to dtype at the end. */
+size_t ddpg_mx_linear_workspace(int64_t M, int64_t K, int64_t N);
 int ddpg_mx_linear(int device, void* stream, int x_dtype, const void* x, int64_t x_row_stride,
-                   int64_t x_col_stride, void* x_codes, void* x_scales, int64_t M, int64_t K,
-                   const void* w_codes, const void* w_scales, int64_t N, int bias_dtype,
-                   const void* bias, int act, int dtype, void* y, int64_t y_row_stride);
+                   int64_t x_col_stride, const void* x_codes, const void* x_scales, int64_t M,
+                   int64_t K, const void* w_codes, const void* w_scales, int64_t N, int bias_dtype,
+                   const void* bias, int act, int dtype, void* y, int64_t y_row_stride, void* ws,
+                   size_t ws_bytes);
 /* Gradients of x . w^T + bias for dy [M, N] of type dtype, with the values the
  * quantised x [M, K] and w [N, K] stand for (straight-through: the quantisation's
  * own derivative is taken as 1): dx [M, K] = dy . w (of type dtype), dw [N, K] =

@@ -87,7 +87,8 @@ def test_mx_entry_refusals():
     lin = lambda **k: L.ddpg_mx_linear(0, None, k.get("xd", 0), k.get("x"), 4, 1, 16, 16,
                                        k.get("M", 4), k.get("K", 4), k.get("w", 16), 16, 4,
                                        k.get("bd", 0), k.get("b"), k.get("act", 0),
-                                       k.get("dt", 0), k.get("y", 16), k.get("ld", 4))
+                                       k.get("dt", 0), k.get("y", 16), k.get("ld", 4),
+                                       k.get("ws"), k.get("nb", 0))
     refused(lin(M=-1), "outside")
     refused(lin(K=big), "outside")
     refused(lin(w=None), "null")
@@ -97,6 +98,10 @@ def test_mx_entry_refusals():
     refused(lin(b=16, bd=4), "dtype 4")
     refused(lin(y=None), "null")
     refused(lin(ld=3), "overlap")
+    refused(lin(M=100, x=16), "workspace")
+    nb = L.ddpg_mx_linear_workspace(100, 4, 4)
+    assert nb == 2 * 4352 and L.ddpg_mx_linear_workspace(1, 4, 4) == 0
+    refused(lin(M=100, x=16, ws=24, nb=nb), "workspace")
     need = L.ddpg_mx_linear_grad_workspace(0, 4, 4, 4, 1, 1, 1)
     assert need > 0 and L.ddpg_mx_linear_grad_workspace(0, 4, 4, 4, 0, 0, 0) == 0
     grad = lambda **k: L.ddpg_mx_linear_grad(0, None, k.get("dt", 0), k.get("dy", 16), 4, 1,
