@@ -42,35 +42,46 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// One block: 32 values to codes and the scale byte.  E = floor(log2 max) - 2 is
-// the exponent field of the largest magnitude less 2 (its bits order like the
-// magnitudes; an infinity or a NaN has the field 255), at least 0: below 2^-125
-// the scale stays 2^-127.  x / 2^E is exact, so v_cvt_scalef32_pk_fp4_f32 makes
-// the one rounding: nearest, ties to the even code, at most 6.
-DDPG_DEV u32x4 mx_quantize_block(const float (&x)[32], unsigned& scale) {
+// The bits of the largest magnitude of n values: bits order like magnitudes, an
+// infinity and a NaN beyond the rest.
+template <int N>
+DDPG_DEV unsigned mx_top(const float* x) {
   unsigned top = 0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  return top;
+}
+// A block's scale byte: E = floor(log2 max) - 2 is the exponent field of the
+// largest magnitude less 2 (255 stays: not finite), at least 0: below 2^-125 the
+// scale stays 2^-127.
+DDPG_DEV unsigned mx_scale_of(unsigned top) {
   const int ef = (int)(top >> 23);
-  scale = ef == 255 ? 255u : (unsigned)max(ef - 2, 0);
-  // 2^(scale - 127); 2^-127 is subnormal
-  const float s = __uint_as_float(scale ? scale << 23 : 0x00400000u);
-  u32x4 q;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    unsigned v = 0;
-    v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[8 * w], x[8 * w + 1], s, 0);
-    v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[8 * w + 2], x[8 * w + 3], s, 1);
-    v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[8 * w + 4], x[8 * w + 5], s, 2);
-    v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[8 * w + 6], x[8 * w + 7], s, 3);
-    q[w] = v;
-  }
-  return q;
+  return ef == 255 ? 255u : (unsigned)max(ef - 2, 0);
+}
+// 2^(s - 127) (2^-127 is subnormal; 255 gives an infinity)
+DDPG_DEV float mx_factor(unsigned s) { return __uint_as_float(s ? s << 23 : 0x00400000u); }
+
+// Eight values to codes.  x / 2^E is exact, so v_cvt_scalef32_pk_fp4_f32 makes the
+// one rounding: nearest, ties to the even code, at most 6.
+DDPG_DEV unsigned mx_codes8(const float* x, float factor) {
+  unsigned v = 0;
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[0], x[1], factor, 0);
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[2], x[3], factor, 1);
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[4], x[5], factor, 2);
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[6], x[7], factor, 3);
+  return v;
+}
+
+// One block: 32 values to codes and the scale byte.
+DDPG_DEV u32x4 mx_quantize_block(const float (&x)[32], unsigned& scale) {
+  scale = mx_scale_of(mx_top<32>(x));
+  const float f = mx_factor(scale);
+  return u32x4{mx_codes8(x, f), mx_codes8(x + 8, f), mx_codes8(x + 16, f), mx_codes8(x + 24, f)};
 }
 
 // The factor of a scale byte as the conversions below take it.
 DDPG_DEV float mx_scale(unsigned s) {
-  return __uint_as_float(s == 255 ? 0x7fc00000u : s ? s << 23 : 0x00400000u);
+  return s == 255 ? __uint_as_float(0x7fc00000u) : mx_factor(s);
 }
 
 // Eight codes to the values they stand for (exact; a NaN scale gives NaN).

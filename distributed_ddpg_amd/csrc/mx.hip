@@ -6,30 +6,81 @@
 namespace ddpg {
 
 // ---------------------------------------------------------------- quantise
-// A block makes one tile of 64 rows x 128 columns, a thread one 32-block of it.
-// ROWS: a wave takes 16 rows and its lanes read along them (16-byte loads where
-// a block's columns are adjacent).  Otherwise a wave takes 32 columns and its
-// lanes 64 rows, so that a load is contiguous where rows are (a matrix in
-// checkpoint order seen turned).  Loads past the matrix are from its last
-// element and count as 0.
+// A block makes one tile of 64 rows x 128 columns.
+//
+// ROWS (a row's values adjacent): a wave takes 16 rows, four at a time, 16 lanes
+// along a row with 8 values each, so that loads are whole lines; the four lanes of
+// a 32-block share its largest magnitude and write its 16 bytes of codes together.
+// Input that is used once goes past the caches.
+//
+// Otherwise a wave takes 32 columns and its lanes 64 rows, so that a load is
+// contiguous where rows are (a matrix in checkpoint order seen turned); blocks
+// that follow each other take rows that follow each other.
+//
+// Loads past the matrix are from its last element and count as 0.
 template <int DT, bool ROWS>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(
     const typename Elem<DT>::type* __restrict__ x, int rows, int cols, long long sr, long long sc,
     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   __shared__ __attribute__((aligned(4))) uint8_t sb[256];
   const int kt = (cols + 127) >> 7, l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int g64 = blockIdx.x / kt, k = blockIdx.x % kt;
-  const int r = ROWS ? w * 16 + (l & 15) : l, kb = ROWS ? l >> 4 : w;
-  const int row = g64 * 64 + r, c0 = k * 128 + kb * 32;
-  unsigned s = 0;
-  if (g64 * 64 + (r & ~15) < rows) {
-    float v[32];
-    mx_load_block<DT>(x + min(row, rows - 1) * sr, sc, ROWS, c0, cols, v);
-    const u32x4 q = mx_quantize_block(v, s);
-    *reinterpret_cast<u32x4*>(codes + mx_code_at(g64 * 4 + (r >> 4), kt, k) +
-                              (kb * 16 + (r & 15)) * 16) = q;
+  const int n64 = (rows + 63) >> 6;
+  const int g64 = ROWS ? blockIdx.x / kt : blockIdx.x % n64;
+  const int k = ROWS ? blockIdx.x % kt : blockIdx.x / n64;
+  if constexpr (ROWS) {
+    constexpr int V = Elem<DT>::V, L = 8 / V;  // loads of 8 values
+    const int g16 = g64 * 4 + w, c0 = k * 128 + (l & 15) * 8;
+    if (g16 * 16 < rows) {
+      float v[4][8];
+      if (c0 + 8 <= cols) {
+        U16B u[4][L];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < L; ++j)
+            u[i][j] = load16<true>(x + min(g16 * 16 + i * 4 + (l >> 4), rows - 1) * sr + c0 + j * V);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < L; ++j) Elem<DT>::widen(u[i][j], v[i] + j * V);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            v[i][j] = (float)x[min(g16 * 16 + i * 4 + (l >> 4), rows - 1) * sr + min(c0 + j, cols - 1)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[i][j] = c0 + j < cols ? v[i][j] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 4 + (l >> 4), kb = (l & 15) >> 2;
+        unsigned top = mx_top<8>(v[i]);
+        // the largest of the block's four lanes (DPP: lanes ^ 1, then ^ 2)
+        top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xf, 0xf, true));
+        top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xf, 0xf, true));
+        const unsigned s = mx_scale_of(top);
+        *reinterpret_cast<unsigned*>(codes + mx_code_at(g16, kt, k) + (kb * 16 + r) * 16 +
+                                     (l & 3) * 4) = mx_codes8(v[i], mx_factor(s));
+        if ((l & 3) == 0) sb[(kb * 16 + r) * 4 + w] = (uint8_t)s;
+      }
+    } else {
+      sb[l * 4 + w] = 0;
+    }
+  } else {
+    const int row = g64 * 64 + l, c0 = k * 128 + w * 32;
+    unsigned s = 0;
+    if (g64 * 64 + (l & ~15) < rows) {
+      float v[32];
+      mx_load_block<DT, true>(x + min(row, rows - 1) * sr, sc, false, c0, cols, v);
+      const u32x4 q = mx_quantize_block(v, s);
+      *reinterpret_cast<u32x4*>(codes + mx_code_at(g64 * 4 + (l >> 4), kt, k) +
+                                (w * 16 + (l & 15)) * 16) = q;
+    }
+    sb[(w * 16 + (l & 15)) * 4 + (l >> 4)] = (uint8_t)s;
   }
-  sb[(kb * 16 + (r & 15)) * 4 + (r >> 4)] = (uint8_t)s;
   __syncthreads();
   if (w == 0)
     reinterpret_cast<unsigned*>(scales + mx_scale_at(g64, kt, k))[l] =

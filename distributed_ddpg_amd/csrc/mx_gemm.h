@@ -570,7 +570,8 @@ struct RawX {
   int vec;  // columns adjacent
 };
 
-template <int DT>
+// NT: past the caches
+template <int DT, bool NT = false>
 DDPG_DEV void mx_load_block(const typename Elem<DT>::type* p, long long sc, bool adjacent, int c0,
                             int cols, float (&v)[32]) {
   if (adjacent && c0 + 32 <= cols) {
@@ -580,7 +581,10 @@ DDPG_DEV void mx_load_block(const typename Elem<DT>::type* p, long long sc, bool
       Elem<DT>::widen(*reinterpret_cast<const U16B*>(p + c0 + i), v + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = (float)p[min(c0 + i, cols - 1) * sc];
+    for (int i = 0; i < 32; ++i) {
+      const typename Elem<DT>::type* q = p + min(c0 + i, cols - 1) * sc;
+      v[i] = (float)(NT ? __builtin_nontemporal_load(q) : *q);
+    }
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = c0 + i < cols ? v[i] : 0.f;
   }

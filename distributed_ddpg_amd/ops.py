@@ -25,6 +25,7 @@ from . import _lib
 from ._lib import lib
 
 _DTYPES = {torch.float32: _lib.FP32, torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
+_STRIDED = {torch.strided}
 _ACTS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "elu": _lib.ACT_ELU, "tanh": _lib.ACT_TANH}
 
 
@@ -87,11 +88,21 @@ class _List:
         self.src = src = [t for t in tensors if t is not None]
         if not src:
             raise ValueError("t_list: no tensor in the list")
-        dt = array("i", [_tensor("t_list", t) for t in src])
-        self.index = src[0].get_device()
-        for t in src:
-            if t.get_device() != self.index:
-                raise ValueError("t_list: tensors on %s and %s" % (src[0].device, t.device))
+        # whole-list checks (a list has hundreds of tensors); what fails one is
+        # named by the tensor's own check
+        try:
+            dt = array("i", [_DTYPES[t.dtype] for t in src])
+            index = {t.get_device() for t in src}
+            fine = (len(index) == 1 and min(index) >= 0 and {t.layout for t in src} == _STRIDED
+                    and not (torch.is_grad_enabled() and any([t.requires_grad for t in src])))
+        except (AttributeError, KeyError, TypeError):
+            fine = False
+        if not fine:
+            for i, t in enumerate(src):
+                _tensor("t_list[%d]" % i, t)
+            raise ValueError("t_list: tensors on %s" % " and ".join(
+                sorted({str(t.device) for t in src})))
+        self.index = index.pop()
         self.kept = src
         cols = ld = None
         if not all([t.is_contiguous() for t in src]):
