@@ -97,6 +97,8 @@ PROTOTYPES = [
     ("ddpg_actor_train", _c.c_int, [_P, _fp, _fp, _c.c_int]),
     ("ddpg_soft_update", _c.c_int, [_P, _c.c_int]),
     ("ddpg_set_scaler", _c.c_int, [_P, _dp, _dp, _c.c_int]),
+    ("ddpg_set_grad_clip", _c.c_int, [_P, _c.c_float, _c.c_float]),
+    ("ddpg_get_grad_norms", _c.c_int, [_P, _fp, _fp]),
     ("ddpg_sampler_create", _c.c_int, [_c.c_int64, _c.POINTER(_P)]),
     ("ddpg_sampler_destroy", None, [_P]),
     ("ddpg_sampler_sample", _c.c_int, [_P, _c.c_int64, _c.c_int, _i64p]),

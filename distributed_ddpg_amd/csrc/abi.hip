@@ -51,7 +51,7 @@ static void ctx_free(ddpg_ctx* c) {
     if (p) (void)hipFree(p);
   for (void* p : {(void*)c->dparams, (void*)c->dpw, (void*)c->dact, (void*)c->d_slots,
                   (void*)c->dmean, (void*)c->dscale, (void*)c->dacc, (void*)c->dstats_all,
-                  (void*)c->xbuf, (void*)c->xrs})
+                  (void*)c->xbuf, (void*)c->xrs, (void*)c->dclip, (void*)c->clip_part})
     if (p) (void)hipFree(p);
   for (auto st : c->aux)
     if (st) (void)hipStreamDestroy(st);
@@ -412,6 +412,37 @@ int ddpg_get_adam_powers(ddpg_ctx* c, int net, float* b1p, float* b2p) {
     HIP_TRY(hipMemcpy(pw, c->dpw + 2 * net, sizeof pw, hipMemcpyDeviceToHost));
     *b1p = pw[0];
     *b2p = pw[1];
+  });
+}
+
+int ddpg_set_grad_clip(ddpg_ctx* c, float actor, float critic) {
+  return guard(c, [&] {
+    const float clip[2] = {actor, critic};
+    if (!(actor >= 0.f) || !(critic >= 0.f))
+      throw einval("gradient clip (%g, %g): norms are numbers >= 0 (0: no clip)", actor, critic);
+    if (!c->dclip) {
+      HIP_TRY(hipMalloc(&c->clip_part, clip_factor_workspace()));
+      HIP_TRY(hipMalloc(&c->dclip, 4 * sizeof(float)));
+      c->grad_clip[0] = c->grad_clip[1] = -1.f;  // neither slot is written yet
+    }
+    HIP_TRY(hipStreamSynchronize(c->stream));
+    for (int net = 0; net < 2; ++net) {
+      const float none[2] = {NAN, 1.f};  // {norm, factor}
+      if (!(clip[net] > 0.f) || !(c->grad_clip[net] > 0.f))
+        HIP_TRY(hipMemcpy(c->dclip + 2 * net, none, sizeof none, hipMemcpyHostToDevice));
+      c->grad_clip[net] = clip[net];
+    }
+  });
+}
+
+int ddpg_get_grad_norms(ddpg_ctx* c, float* actor, float* critic) {
+  return guard(c, [&] {
+    if (!c->dclip) throw DdpgError(DDPG_ESTATE, "no gradient clip was set (ddpg_set_grad_clip)");
+    float v[4];
+    HIP_TRY(hipMemcpyAsync(v, c->dclip, sizeof v, hipMemcpyDeviceToHost, c->stream));
+    HIP_TRY(hipStreamSynchronize(c->stream));
+    if (actor) *actor = v[0];
+    if (critic) *critic = v[2];
   });
 }
 

@@ -197,6 +197,11 @@ struct ddpg_ctx {
   double* dacc = nullptr;        // [qmax_sum, loss_sum, steps]
   double *dmean = nullptr, *dscale = nullptr;
   bool has_scaler = false;
+  // ddpg_set_grad_clip: per network (0 actor, 1 critic) the largest gradient
+  // norm (0: no clip); dclip[2 net] = {norm, factor} of the last update
+  float grad_clip[2] = {0.f, 0.f};
+  float* dclip = nullptr;
+  double* clip_part = nullptr;  // partial sums
 
   // activations / workspaces
   float* dact = nullptr;
@@ -241,6 +246,7 @@ struct ddpg_ctx {
     int B = -1;
     const void* rb = nullptr;
     bool scaler = false;
+    float clip[2] = {0.f, 0.f};
     int* h_idx = nullptr;
     hipEvent_t done = nullptr;
   } gslot[2];
@@ -470,6 +476,10 @@ GemmPlan wgrad_launch(ddpg_ctx* c, const float* A, int lda, const float* B, int 
                       int K, float* slab, int cap, float* direct);
 // step.hip
 void sb_setup(ddpg_ctx* c);  // ddpg_create: small-batch path eligibility and buffers
+// norm.hip
+void clip_factor_launch(hipStream_t st, const float* g, long long n, float clip, double* part,
+                        float* out);
+size_t clip_factor_workspace();
 // dp.hip
 void allreduce_on_cs(ddpg_ctx* c, int ev, const char* name, float* b0, size_t n0,
                      float* b1 = nullptr, size_t n1 = 0, bool with_stats = false,

@@ -524,6 +524,8 @@ __global__ __launch_bounds__(256) void reduce_slabs_kernel(ReduceTable tab) {
 // updated from the new p in the same pass (networks.py:34-37, the same fp32
 // ops as soft_update_kernel; nothing reads the targets between this network's
 // Adam step and the end of the step), ttw its twin.
+// gscale (optional): the clip's factor; the gradient is scaled by it first, in
+// its buffer too (what ddpg_get_params returns is what the update applied).
 // alpha = lr * sqrt(1 - b2p) / (1 - b1p) from a network's beta powers
 DDPG_DEV float adam_alpha(const float* pw, float lr) {
   return __fdiv_rn(__fmul_rn(lr, __fsqrt_rn(__fsub_rn(1.f, pw[1]))), __fsub_rn(1.f, pw[0]));
@@ -557,13 +559,15 @@ DDPG_DEV void adam_hooks(const AdamHooks& h, float b1, float b2) {
 }
 
 __global__ void adam_kernel(float* __restrict__ p, float* __restrict__ m,
-                            float* __restrict__ v, const float* __restrict__ g, long long n,
+                            float* __restrict__ v, float* __restrict__ g, long long n,
                             const float* __restrict__ pw, float lr, float b1, float b2,
                             float eps, __bf16* __restrict__ tw, long long tps, int tnp,
                             float* __restrict__ tt, float tau, float omt,
-                            __bf16* __restrict__ ttw, AdamHooks hk) {
+                            __bf16* __restrict__ ttw, AdamHooks hk, const float* gscale) {
   const float alpha = hk.alpha_in ? *hk.alpha_in : adam_alpha(pw, lr);
   adam_hooks(hk, b1, b2);
+  const float gs = gscale ? *gscale : 1.f;
+  const bool clipped = gs != 1.f;  // grid-uniform
   const float omb1 = __fsub_rn(1.f, b1), omb2 = __fsub_rn(1.f, b2);
   const long long n4 = n >> 2;
   const long long stride = (long long)gridDim.x * blockDim.x;
@@ -571,7 +575,14 @@ __global__ void adam_kernel(float* __restrict__ p, float* __restrict__ m,
     float4 P = reinterpret_cast<float4*>(p)[i];
     float4 Mv = reinterpret_cast<float4*>(m)[i];
     float4 V = reinterpret_cast<const float4*>(v)[i];
-    const float4 G = reinterpret_cast<const float4*>(g)[i];
+    float4 G = reinterpret_cast<const float4*>(g)[i];
+    if (clipped) {
+      G.x = __fmul_rn(G.x, gs);
+      G.y = __fmul_rn(G.y, gs);
+      G.z = __fmul_rn(G.z, gs);
+      G.w = __fmul_rn(G.w, gs);
+      reinterpret_cast<float4*>(g)[i] = G;
+    }
     float* pp = &P.x;
     float* pm = &Mv.x;
     float* pv = &V.x;
@@ -600,6 +611,7 @@ __global__ void adam_kernel(float* __restrict__ p, float* __restrict__ m,
   // tail (n % 4)
   if (blockIdx.x == 0 && threadIdx.x < (n & 3)) {
     const long long i = (n4 << 2) + threadIdx.x;
+    if (clipped) g[i] = __fmul_rn(g[i], gs);
     m[i] = __fadd_rn(m[i], __fmul_rn(__fsub_rn(g[i], m[i]), omb1));
     v[i] = __fadd_rn(v[i], __fmul_rn(__fsub_rn(__fmul_rn(g[i], g[i]), v[i]), omb2));
     p[i] = __fsub_rn(p[i], __fdiv_rn(__fmul_rn(m[i], alpha), __fadd_rn(__fsqrt_rn(v[i]), eps)));

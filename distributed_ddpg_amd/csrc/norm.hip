@@ -109,10 +109,20 @@ DDPG_DEV double gn_total(const double* part, int np, double* red) {
   return sqrt(block_sum(s, red));
 }
 
-__global__ __launch_bounds__(GN_T) void gn_norm_kernel(const double* part, int np, float* norm) {
+// NaN stays NaN, an infinite norm leaves 0
+DDPG_DEV double gn_factor(double n, float clip) {
+  return n <= (double)clip ? 1.0 : (double)clip / n;
+}
+
+// scale (optional): the clip's factor beside the norm
+__global__ __launch_bounds__(GN_T) void gn_norm_kernel(const double* part, int np, float* norm,
+                                                       float clip, float* scale) {
   __shared__ double red[GN_T / 64];
   const double n = gn_total(part, np, red);
-  if (threadIdx.x == 0) *norm = (float)n;
+  if (threadIdx.x == 0) {
+    *norm = (float)n;
+    if (scale) *scale = (float)gn_factor(n, clip);
+  }
 }
 
 // y = x * s: the float32 product of a float64 scale, rounded once.  given:
@@ -123,7 +133,7 @@ __global__ __launch_bounds__(GN_T) void gn_scale_kernel(GnTable t, const double*
   __shared__ double red[GN_T / 64];
   const double n = given ? (double)*given : gn_total(part, np, red);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-  const double s = n <= (double)clip ? 1.0 : (double)clip / n;  // NaN stays NaN
+  const double s = gn_factor(n, clip);
   gn_chunks<true>(t, [&](auto dt, const GnEntry& e, long long i0, int m, int c) {
     typedef Elem<dt.value> E;
     constexpr int V = E::V;
@@ -265,6 +275,20 @@ static int gn_partials(const GnList& l, bool again, hipStream_t st, double* part
 
 }  // namespace ddpg
 
+// A learner's gradient before its Adam pass (step.hip): out[0] = the norm of the
+// n values at g, out[1] = the factor that clips it.
+void clip_factor_launch(hipStream_t st, const float* g, long long n, float clip, double* part,
+                        float* out) {
+  const int dtype = T_FP32;
+  const void* src = g;
+  const int64_t count = n;
+  const GnList l{1, &dtype, &src, nullptr, &count, nullptr, nullptr};
+  const int np = gn_partials(l, true, st, part, gn_ws(1));
+  hipLaunchKernelGGL(gn_norm_kernel, dim3(1), dim3(GN_T), 0, st, part, np, out, clip, out + 1);
+  HIP_TRY(hipGetLastError());
+}
+size_t clip_factor_workspace() { return gn_ws(1); }
+
 extern "C" {
 
 size_t ddpg_global_norm_workspace(int n) { return gn_ws(n); }
@@ -280,7 +304,8 @@ int ddpg_global_norm(int device, void* stream, int n, const int* dtype, const vo
     const hipStream_t st = static_cast<hipStream_t>(stream);
     double* part = static_cast<double*>(ws);
     const int np = gn_partials(l, false, st, part, ws_bytes);
-    hipLaunchKernelGGL(gn_norm_kernel, dim3(1), dim3(GN_T), 0, st, part, np, norm);
+    hipLaunchKernelGGL(gn_norm_kernel, dim3(1), dim3(GN_T), 0, st, part, np, norm, 0.f,
+                       nullptr);
     HIP_TRY(hipGetLastError());
   });
 }
@@ -310,7 +335,8 @@ int ddpg_clip_by_global_norm(int device, void* stream, int n, const int* dtype,
       first = false;
     });
     if (first && !use_norm) {  // no element anywhere: the norm is 0
-      hipLaunchKernelGGL(gn_norm_kernel, dim3(1), dim3(GN_T), 0, st, part, 0, norm);
+      hipLaunchKernelGGL(gn_norm_kernel, dim3(1), dim3(GN_T), 0, st, part, 0, norm, 0.f,
+                         nullptr);
       HIP_TRY(hipGetLastError());
     }
   });

@@ -94,6 +94,7 @@ struct SbArgs {
   float* alpha;          // [actor, critic] Adam step sizes for this step
   float* stats;          // [q_max, loss]
   double* acc;           // [qmax_sum, loss_sum, steps]
+  const float* clip[2];  // per network: the clip's factor of this update, or null
   long long aW1, ab1, aW2, ab2, aW3;
   long long cWs, cbs, cWa, cba, cWh, cbh, cWo, cbo;
 #ifdef DDPG_SB_STAMPS
@@ -763,7 +764,10 @@ constexpr int SB_GSJ = (SB_GROWS * 16 + SB_GT - 1) / SB_GT;  // staged float4s p
 // RCCL sum of the gradient buffer: mode 1 computes and stores this rank's
 // gradient only (the critic call stores this rank's {max Q, loss share} to
 // g.stats for the all-gather, no running sums); mode 2 reads the summed
-// gradient back and applies Adam, the soft update and the shadow.
+// gradient back and applies Adam, the soft update and the shadow.  A clipped
+// gradient without an exchange takes the same two launches around its norm: mode
+// 3 is mode 1 with the running sums kept as in mode 0, and mode 2 scales by the
+// clip's factor (g.clip), in the gradient buffer too.
 //
 // The critic's call forms dQ = -((1/B) * (2 * (y - q))) per row (the MSE
 // gradient, networks.py:136, from phase 1's saved q and TD target) into LDS
@@ -797,7 +801,8 @@ __global__ __launch_bounds__(SB_GT) void sb_wgrad_adam_kernel(SbArgs g, SbGradTa
   const int kc = min(k, T.K - 1), nc = min(n, T.N - 1);
   const size_t i = (size_t)T.off + (size_t)kc * T.N + nc;
   float m0 = 0.f, v0 = 0.f, p0 = 0.f, t0 = 0.f;
-  if (mode != 1) {
+  const bool grad_only = mode == 1 || mode == 3;
+  if (!grad_only) {
     m0 = g.adam_m[i];
     v0 = g.adam_v[i];
     p0 = g.theta[i];
@@ -812,6 +817,13 @@ __global__ __launch_bounds__(SB_GT) void sb_wgrad_adam_kernel(SbArgs g, SbGradTa
   const int nB = mode == 2 ? 0 : g.B;
   lds_f* const st = LDS(stg);
   float gv = mode == 2 ? g.grad[i] : 0.f;
+  if (mode == 2 && g.clip[net]) {
+    const float gs = *g.clip[net];
+    if (gs != 1.f) {
+      gv = __fmul_rn(gv, gs);
+      if (ok) g.grad[i] = gv;
+    }
+  }
   for (int b0 = 0; b0 < nB; b0 += SB_GC) {
     const int nq4 = (min(SB_GC, nB - b0) + 3) >> 2;  // float4s per staged row
     // a thread stages quad qd of every row it touches (SB_GT is a multiple
@@ -885,8 +897,8 @@ __global__ __launch_bounds__(SB_GT) void sb_wgrad_adam_kernel(SbArgs g, SbGradTa
     __syncthreads();  // the next chunk's stores reuse the tile
   }
   SB_STAMP(sbase + 1);
-  if (ok && mode == 1) g.grad[i] = gv;
-  if (ok && mode != 1) {
+  if (ok && grad_only) g.grad[i] = gv;
+  if (ok && !grad_only) {
     const float alpha = g.alpha[net];
     const float omb1 = __fsub_rn(1.f, g.b1), omb2 = __fsub_rn(1.f, g.b2);
     const float m = __fadd_rn(m0, __fmul_rn(__fsub_rn(gv, m0), omb1));
@@ -910,7 +922,7 @@ __global__ __launch_bounds__(SB_GT) void sb_wgrad_adam_kernel(SbArgs g, SbGradTa
     const float loss = __fmul_rn(ls, g.inv_b);
     g.stats[0] = qm;
     g.stats[1] = loss;
-    if (mode == 0) {  // mode 1: the data-parallel stats reduction keeps the sums
+    if (mode == 0 || mode == 3) {  // mode 1: the data-parallel stats reduction keeps the sums
       g.acc[0] += (double)qm;
       g.acc[1] += (double)loss;
       g.acc[2] += 1.0;

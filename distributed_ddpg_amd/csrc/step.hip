@@ -338,7 +338,20 @@ static AdamHooks adam_hooks_for(ddpg_ctx* c, int net, bool fold) {
   return h;
 }
 
+// The clip's factor of a network's (summed) gradient, for its Adam pass; null
+// without a clip.
+static const float* clip_launch(ddpg_ctx* c, int net) {
+  if (!(c->grad_clip[net] > 0.f)) return nullptr;
+  const size_t b = net == 0 ? c->L.actor_begin : c->L.critic_begin;
+  const size_t e = net == 0 ? c->L.actor_end : c->L.critic_end;
+  ProfScope ps(c, "grad_norm", 2.0 * (e - b), 4.0 * (e - b));
+  clip_factor_launch(c->cur, c->grad + b, (long long)(e - b), c->grad_clip[net], c->clip_part,
+                     c->dclip + 2 * net);
+  return c->dclip + 2 * net + 1;
+}
+
 static void adam_launch(ddpg_ctx* c, int net, bool advance, bool soft = false) {
+  const float* gscale = clip_launch(c, net);
   const size_t b = net == 0 ? c->L.actor_begin : c->L.critic_begin;
   const size_t e = net == 0 ? c->L.actor_end : c->L.critic_end;
   const long long n = (long long)(e - b);
@@ -355,7 +368,7 @@ static void adam_launch(ddpg_ctx* c, int net, bool advance, bool soft = false) {
                        c->adam_m + b, c->adam_v + b, c->grad + b, n, c->dpw + 2 * net, lr,
                        c->cfg.beta1, c->cfg.beta2, c->cfg.epsilon, tw, (long long)c->L.total,
                        c->hnp, soft ? c->target + b : nullptr, tau, omt, soft ? ttw : nullptr,
-                       adam_hooks_for(c, net, soft));
+                       adam_hooks_for(c, net, soft), gscale);
     HIP_TRY(hipGetLastError());
   }
   if (advance) {
@@ -640,7 +653,7 @@ static void critic_train_dev(ddpg_ctx* c, int B, float inv_b, bool fused, int nq
   add_seg(tab, part_dbh, G + L.c[CBH].off, c->CH2, nchunk, c->CH2);
   add_seg(tab, part_dWo, G + L.c[CWO].off, c->CH2, nchunk, c->CH2);
   add_seg(tab, part_dbo, G + L.c[CBO].off, 1, nchunk, 1);
-  if (!c->comm) {
+  if (!c->comm && !(c->grad_clip[1] > 0.f)) {
     adam_reduce_launch(c, 1, tab, !fused, fused);
     return;
   }
@@ -796,12 +809,12 @@ static void actor_train_dev(ddpg_ctx* c, int B, bool fused, bool par = false) {
             (long long)c->AH2 * c->A);
   else
     add_wgrad(tab, pW3, c->slab_W3, G + L.a[AW3].off, (long long)c->AH2 * c->A);
-  if (!c->comm) {
+  if (!c->comm && !(c->grad_clip[0] > 0.f)) {
     adam_reduce_launch(c, 0, tab, !fused, fused);
     return;
   }
   reduce_launch(c, "grad_reduce", tab);
-  {  // [W1 b1] and [b2 W3] behind dW2 on the comm stream
+  if (c->comm) {  // [W1 b1] and [b2 W3] behind dW2 on the comm stream
     allreduce_on_cs(c, 4, "rccl_allreduce", G + L.actor_begin, L.a[AW2].off - L.actor_begin,
                     G + L.a[AB2].off, L.actor_end - L.a[AB2].off, false, "xwin|actor_tail");
     join_cs(c, 5);
@@ -1020,6 +1033,8 @@ static SbArgs sb_args(ddpg_ctx* c, ddpg_replay* rb, int B, float inv_b) {
   a.alpha = c->sb_misc;
   a.stats = c->dstats;
   a.acc = c->dacc;
+  for (int net = 0; net < 2; ++net)
+    a.clip[net] = c->grad_clip[net] > 0.f ? c->dclip + 2 * net + 1 : nullptr;
   a.aW1 = L.a[AW1].off;
   a.ab1 = L.a[AB1].off;
   a.aW2 = L.a[AW2].off;
@@ -1075,7 +1090,11 @@ static void learner_step_small(ddpg_ctx* c, ddpg_replay* rb, int B, float inv_b)
     hipLaunchKernelGGL(sb_phase1_kernel, dim3(grid), dim3(SB_NT), c->sb_smem, c->cur, a);
     HIP_TRY(hipGetLastError());
   }
-  if (!dp) {
+  if (!dp && a.clip[1]) {
+    sb_wgrad(c, a, 1, G, 3, (double)nc);
+    clip_launch(c, 1);
+    sb_wgrad(c, a, 1, G, 2, (double)nc);
+  } else if (!dp) {
     sb_wgrad(c, a, 1, G, 0, (double)nc);
   } else {
     sb_wgrad(c, a, 1, G, 1, (double)nc);
@@ -1083,6 +1102,7 @@ static void learner_step_small(ddpg_ctx* c, ddpg_replay* rb, int B, float inv_b)
                     nullptr);
     stats_allreduce_on_cs(c, true);
     join_cs(c, 2);
+    clip_launch(c, 1);
     sb_wgrad(c, a, 1, G, 2, (double)nc);
   }
   {
@@ -1092,13 +1112,18 @@ static void learner_step_small(ddpg_ctx* c, ddpg_replay* rb, int B, float inv_b)
     hipLaunchKernelGGL(sb_phase3_kernel, dim3(G * a.xstride), dim3(SB_NT), c->sb_smem, c->cur, a);
     HIP_TRY(hipGetLastError());
   }
-  if (!dp) {
+  if (!dp && a.clip[0]) {
+    sb_wgrad(c, a, 0, G, 3, (double)na);
+    clip_launch(c, 0);
+    sb_wgrad(c, a, 0, G, 2, (double)na);
+  } else if (!dp) {
     sb_wgrad(c, a, 0, G, 0, (double)na);
   } else {
     sb_wgrad(c, a, 0, G, 1, (double)na);
     allreduce_on_cs(c, 4, "rccl_allreduce", Gb + L.actor_begin, (size_t)na, nullptr, 0, false,
                     nullptr);
     join_cs(c, 5);
+    clip_launch(c, 0);
     sb_wgrad(c, a, 0, G, 2, (double)na);
   }
 }
@@ -1534,7 +1559,8 @@ static void step_common(ddpg_ctx* c, ddpg_replay* rb, const int64_t* idx, int Bg
     auto& g = c->gslot[c->gcur];
     HIP_TRY(hipEventSynchronize(g.done));  // this slot's previous replay has finished
     for (int i = 0; i < B; ++i) g.h_idx[i] = pos_to_slot(rb, mine[i]);
-    if (!g.exec || g.B != B || g.rb != rb || g.scaler != c->has_scaler) {
+    if (!g.exec || g.B != B || g.rb != rb || g.scaler != c->has_scaler ||
+        g.clip[0] != c->grad_clip[0] || g.clip[1] != c->grad_clip[1]) {
       if (g.exec) HIP_TRY(hipGraphExecDestroy(g.exec));
       g.exec = nullptr;
       hipGraph_t graph = nullptr;
@@ -1583,6 +1609,8 @@ static void step_common(ddpg_ctx* c, ddpg_replay* rb, const int64_t* idx, int Bg
         g.B = B;
         g.rb = rb;
         g.scaler = c->has_scaler;
+        g.clip[0] = c->grad_clip[0];
+        g.clip[1] = c->grad_clip[1];
       }
     }
     if (g.exec) {

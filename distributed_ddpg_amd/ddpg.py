@@ -153,7 +153,7 @@ def run_worker(opt, task_index, env_name, episodes, device):
     critic = nets.CriticNetwork(S, A, opt.critic_lr, opt.tau, actor.get_num_trainable_vars(),
                                 scaler, h1=H1, h2=H2)
     sess = nets.Session(device=device, batch_max=max(opt.batch_size // world, 1), rank=rank,
-                        world=world)
+                        world=world, grad_clip=opt.grad_clip)
     sess.run(nets.global_variables_initializer(seed=opt.seed))
     actor.set_session(sess)
     critic.set_session(sess)

@@ -56,15 +56,26 @@ def global_variables_initializer(seed=1234):
     return _InitOp(seed)
 
 
+def _clip_norm(x):
+    """A clip as the C call takes it: 0 for none."""
+    if x is None:
+        return 0.0
+    if not x > 0:
+        raise ValueError("gradient clip %r is not a norm > 0 (None: no clip)" % (x,))
+    return float(x)
+
+
 class Session:
     """tf.Session stand-in owning one device context (one per process/GPU).
 
     Session(target=None, graph=None, device=0, batch_max=4096, rank=0, world=1)
     `target` (the reference's server.target) is accepted and ignored.
+    grad_clip: largest global norm of each network's gradient (a number, or
+    (actor, critic) with None for no clip): see set_grad_clip.
     """
 
     def __init__(self, target=None, graph=None, device=0, batch_max=4096, rank=0, world=1,
-                 dtype="fp32"):
+                 dtype="fp32", grad_clip=None):
         g = graph or _default_graph
         if g.actor is None or g.critic is None:
             raise ValueError("build ActorNetwork and CriticNetwork before opening a Session")
@@ -89,7 +100,14 @@ class Session:
         cfg.device, cfg.rank, cfg.world = int(device), int(rank), int(world)
         self.cfg = cfg
         self.ctx = _lib.ctypes.c_void_p()
+        clip = grad_clip if isinstance(grad_clip, (list, tuple)) else (grad_clip, grad_clip)
+        clip = [_clip_norm(x) for x in clip]
+        if len(clip) != 2:
+            raise ValueError("grad_clip: expected a number or (actor, critic), got %r" % (
+                grad_clip,))
         check(lib.ddpg_create(_lib.ctypes.byref(cfg), _lib.ctypes.byref(self.ctx)))
+        if any(clip):
+            check(lib.ddpg_set_grad_clip(self.ctx, *clip), self.ctx)
         # action selection's host staging: ctypes arrays passed as they are
         # (numpy's .ctypes pointer conversion costs microseconds per call)
         self._io_in = (_lib.ctypes.c_float * _IO_FLOATS)()
@@ -168,6 +186,21 @@ class Session:
         a, b = _lib.ctypes.c_float(), _lib.ctypes.c_float()
         check(lib.ddpg_get_adam_powers(self.ctx, net, _lib.ctypes.byref(a),
                                        _lib.ctypes.byref(b)), self.ctx)
+        return a.value, b.value
+
+    def set_grad_clip(self, actor=None, critic=None):
+        """Clip each network's gradient by its global norm before Adam
+        (tf.clip_by_global_norm between compute_gradients and apply_gradients),
+        in the fused step and in train(): the largest norm per network, None for
+        no clip, inf to have grad_norms() only."""
+        check(lib.ddpg_set_grad_clip(self.ctx, _clip_norm(actor), _clip_norm(critic)), self.ctx)
+
+    def grad_norms(self):
+        """(actor, critic) gradient norms of the last update, before the clip; NaN
+        for a network without one."""
+        a, b = _lib.ctypes.c_float(), _lib.ctypes.c_float()
+        check(lib.ddpg_get_grad_norms(self.ctx, _lib.ctypes.byref(a), _lib.ctypes.byref(b)),
+              self.ctx)
         return a.value, b.value
 
     def sync(self):

@@ -35,4 +35,5 @@ class Parameters:
 
         # MI355X build additions (not in the reference)
         self.hidden = (128, 200)        # networks.py:54-55,151-156
+        self.grad_clip = None           # largest gradient norm (a number or (actor, critic))
         self.device = 0

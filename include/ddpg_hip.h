@@ -147,6 +147,16 @@ int ddpg_soft_update(ddpg_ctx* ctx, int mask);
  * the reference's feed_dict received them.  NULL clears. */
 int ddpg_set_scaler(ddpg_ctx* ctx, const double* mean, const double* scale, int S);
 
+/* Clip each network's gradient by its global norm between the gradient (after
+ * the data-parallel sum) and Adam, in the fused step and the 1:1 train calls: g *
+ * min(1, clip / norm), i.e. tf.clip_by_global_norm over compute_gradients'
+ * list.  Per network the largest norm; 0 (the default) switches the clip off,
+ * INFINITY computes the norm only.  DDPG_*_GRAD returns the clipped gradient. */
+int ddpg_set_grad_clip(ddpg_ctx* ctx, float actor, float critic);
+/* The norms (before the clip) of the last update; NaN for a network without a
+ * clip.  DDPG_ESTATE if ddpg_set_grad_clip was never called.  Synchronises. */
+int ddpg_get_grad_norms(ddpg_ctx* ctx, float* actor, float* critic);
+
 /* ------------------------------------------------------------- replay */
 /* Host restatement of CPython random.seed(int) + random.sample (MT19937),
  * the sampler behind ReplayBuffer.sample_batch (replay_buffer.py:19,33-39). */
