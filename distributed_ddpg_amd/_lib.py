@@ -95,6 +95,9 @@ PROTOTYPES = [
     ("ddpg_critic_train", _c.c_int, [_P, _fp, _fp, _fp, _c.c_int, _fp, _fp]),
     ("ddpg_critic_action_grad", _c.c_int, [_P, _fp, _fp, _c.c_int, _fp]),
     ("ddpg_actor_train", _c.c_int, [_P, _fp, _fp, _c.c_int]),
+    ("ddpg_actor_publish_mx", _c.c_int, [_P, _c.c_int]),
+    ("ddpg_actor_forward_mx", _c.c_int, [_P, _fp, _c.c_int, _fp]),
+    ("ddpg_actor_train_mx", _c.c_int, [_P, _fp, _fp, _c.c_int]),
     ("ddpg_soft_update", _c.c_int, [_P, _c.c_int]),
     ("ddpg_set_scaler", _c.c_int, [_P, _dp, _dp, _c.c_int]),
     ("ddpg_set_grad_clip", _c.c_int, [_P, _c.c_float, _c.c_float]),

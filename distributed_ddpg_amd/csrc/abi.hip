@@ -45,6 +45,10 @@ static void ctx_free(ddpg_ctx* c) {
     if (g.done) (void)hipEventDestroy(g.done);
   }
   if (c->step_done) (void)hipEventDestroy(c->step_done);
+  for (void* p : {(void*)c->mx.snap, (void*)c->mx.w2, (void*)c->mx.w2_train, (void*)c->mx.xq,
+                  (void*)c->mx.h1, (void*)c->mx.h2, (void*)c->mx.dh1, (void*)c->mx.dw,
+                  (void*)c->mx.ws})
+    if (p) (void)hipFree(p);
   for (void* p : {(void*)c->sb_save, (void*)c->sb_misc, (void*)c->sb_whT, (void*)c->sb_w2T})
     if (p) (void)hipFree(p);
   for (void* p : {(void*)c->atw, (void*)c->wtw, (void*)c->kc_part, (void*)c->kc_ticket})

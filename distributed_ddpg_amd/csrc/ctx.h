@@ -203,6 +203,22 @@ struct ddpg_ctx {
   float* dclip = nullptr;
   double* clip_part = nullptr;  // partial sums
 
+  // The 4-bit policy (ddpg_actor_publish_mx ..), allocated at its first use: a
+  // snapshot of the actor with its hidden layer W2 in MXFP4, and the buffers of
+  // the calls that run it
+  struct {
+    float* snap = nullptr;     // the actor's flat region
+    uint8_t* w2 = nullptr;     // snap's W2^T, quantised
+    bool published = false;
+    uint8_t* w2_train = nullptr;  // the training call's
+    uint8_t* xq = nullptr;     // h1, quantised
+    float* h1 = nullptr;       // [Bmax][ldAH1]
+    float* h2 = nullptr;       // [Bmax][ldAH2]
+    float* dh1 = nullptr;      // [Bmax][AH1]
+    float* dw = nullptr;       // [AH2][AH1]
+    uint8_t* ws = nullptr;     // the gradient's workspace
+  } mx;
+
   // activations / workspaces
   float* dact = nullptr;
   float *s, *s2, *a, *r, *t, *y, *q, *dq;
@@ -480,6 +496,20 @@ void sb_setup(ddpg_ctx* c);  // ddpg_create: small-batch path eligibility and bu
 void clip_factor_launch(hipStream_t st, const float* g, long long n, float clip, double* part,
                         float* out);
 size_t clip_factor_workspace();
+// mx.hip: MXFP4 layers on fp32 buffers (a quantised matrix is one buffer)
+namespace ddpg {
+size_t mx_bytes(int rows, int cols);
+// x's rows and columns sr and sc floats apart
+void mx_quantize_f32(hipStream_t st, const float* x, int rows, int cols, long long sr, long long sc,
+                     uint8_t* q);
+// y = act(x w^T + bias); xq: scratch, or x's quantised form afterwards (keep)
+void mx_layer_f32(hipStream_t st, const float* x, int ldx, int M, int K, const uint8_t* w, int N,
+                  const float* bias, int act, float* y, int ldy, uint8_t* xq, bool keep);
+// dx [M][K], dw [N][K] of a layer whose operands are xq and w (straight-through)
+size_t mx_layer_grad_ws(int M, int N, int K);
+void mx_layer_grad_f32(hipStream_t st, const float* dy, int lddy, int M, int N, int K,
+                       const uint8_t* xq, const uint8_t* w, float* dx, float* dw, uint8_t* ws);
+}  // namespace ddpg
 // dp.hip
 void allreduce_on_cs(ddpg_ctx* c, int ev, const char* name, float* b0, size_t n0,
                      float* b1 = nullptr, size_t n1 = 0, bool with_stats = false,

@@ -178,6 +178,45 @@ __global__ void actor_out_kernel(const float* __restrict__ part, int NT, int B, 
   if (mu) mu[(size_t)b * ld + a] = __fmul_rn(ov, scale);
 }
 
+// part[b][a] = sum_k h[b][k] W[k][a]: a wave per row, the output layer of the
+// 4-bit policy (its h comes from a product without this file's epilogues).
+__global__ __launch_bounds__(256) void project_kernel(const float* __restrict__ h, int ld, int K,
+                                                      const float* __restrict__ W, int A, int B,
+                                                      float* __restrict__ part) {
+  const int b = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
+  if (b >= B) return;
+  for (int a = 0; a < A; ++a) {
+    float s = 0.f;
+#pragma unroll 4
+    for (int k = l; k < K; k += 64) s = fmaf(h[(size_t)b * ld + k], W[(size_t)k * A + a], s);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+    if (l == 0) part[(size_t)b * A + a] = s;
+  }
+}
+
+// dz[b][j] = dh[b][j] elu'(h[b][j]) and each 64-row block's column sums: the
+// 4-bit policy's dz1.
+__global__ __launch_bounds__(256) void elu_grad_kernel(const float* __restrict__ dh, int ldd,
+                                                       const float* __restrict__ h, int ldh, int B,
+                                                       int N, float* __restrict__ dz, int ldz,
+                                                       float* __restrict__ part) {
+  __shared__ float red[4][64];
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, j = blockIdx.x * 64 + l;
+  const int b0 = blockIdx.y * 64;
+  float s = 0.f;
+  if (j < N)
+    for (int b = b0 + w; b < min(b0 + 64, B); b += 4) {
+      const float v = __fmul_rn(dh[(size_t)b * ldd + j], elu_grad_factor(h[(size_t)b * ldh + j]));
+      dz[(size_t)b * ldz + j] = v;
+      s += v;
+    }
+  red[w][l] = s;
+  __syncthreads();
+  if (w == 0 && j < N)
+    part[(size_t)blockIdx.y * N + j] = ((red[0][l] + red[1][l]) + red[2][l]) + red[3][l];
+}
+
 // critic output q = sum_t qpart[t][b] + bo, then by mode:
 //   mode 0: q only;  mode 1: TD target y = t ? r : r + gamma*q  (ddpg.py:92-100)
 __global__ void critic_q_kernel(const float* __restrict__ qpart, int NT, int B,

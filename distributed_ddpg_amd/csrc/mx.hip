@@ -488,6 +488,35 @@ void mx_linear_grad_launch(hipStream_t st, int dtype, const void* dy, long long 
   mx_gemm_launch<false>(st, p, L.pick);
 }
 
+// ---------------------------------------------------------------- the learner's
+// A quantised matrix in one buffer, the scales behind the codes.
+size_t mx_bytes(int rows, int cols) { return mx_code_bytes(rows, cols) + mx_scale_bytes(rows, cols); }
+static MxMat mx_in(const uint8_t* q, int rows, int cols) {
+  return {q, q + mx_code_bytes(rows, cols), rows, cols};
+}
+void mx_quantize_f32(hipStream_t st, const float* x, int rows, int cols, long long sr, long long sc,
+                     uint8_t* q) {
+  mx_quantize_launch(st, T_FP32, x, rows, cols, sr, sc, q, q + mx_code_bytes(rows, cols));
+}
+void mx_layer_f32(hipStream_t st, const float* x, int ldx, int M, int K, const uint8_t* w, int N,
+                  const float* bias, int act, float* y, int ldy, uint8_t* xq, bool keep) {
+  const MxOut o{y, bias, ldy, M, N, T_FP32, T_FP32, act, 0};
+  if (!keep && mx_rows_ok(M, K)) {
+    mx_linear_rows_launch(st, T_FP32, x, ldx, 1, M, K, mx_in(w, N, K), o);
+    return;
+  }
+  mx_quantize_f32(st, x, M, K, ldx, 1, xq);
+  mx_linear_launch(st, mx_in(xq, M, K), mx_in(w, N, K), o);
+}
+size_t mx_layer_grad_ws(int M, int N, int K) {
+  return mx_grad_plan(T_FP32, M, N, K, true, true, false).total;
+}
+void mx_layer_grad_f32(hipStream_t st, const float* dy, int lddy, int M, int N, int K,
+                       const uint8_t* xq, const uint8_t* w, float* dx, float* dw, uint8_t* ws) {
+  mx_linear_grad_launch(st, T_FP32, dy, lddy, 1, mx_in(xq, M, K), mx_in(w, N, K), dx, dw, nullptr,
+                        ws);
+}
+
 }  // namespace ddpg
 
 extern "C" {

@@ -675,7 +675,10 @@ static void critic_train_dev(ddpg_ctx* c, int B, float inv_b, bool fused, int nq
 // Actor update given dz3 (= TanhGrad chain of -dQ/da) and the forward
 // activations h1, h2 of c->s.  networks.py:39-47,71-75.
 // par: weight-gradient GEMMs (dW3, dW2) run on aux[0] beside the dX chain.
-static void actor_train_dev(ddpg_ctx* c, int B, bool fused, bool par = false) {
+// mx: h1 and W2 are the 4-bit policy's (c->mx.h1, quantised c->mx.xq and
+// c->mx.w2_train): the hidden layer's two products are its straight-through
+// gradient.
+static void actor_train_dev(ddpg_ctx* c, int B, bool fused, bool par = false, bool mx = false) {
   const Layout& L = c->L;
   float* G = c->grad;
   const hipStream_t main = c->cur;
@@ -698,7 +701,7 @@ static void actor_train_dev(ddpg_ctx* c, int B, bool fused, bool par = false) {
   // on the twin GEMM
   int kh;
   const Twin dz2t =
-      (gemm_h_ok<L_KR, L_KR>(c, c->h1, c->ldAH1, c->dz2, c->ldAH2, c->AH1, c->AH2, B, 0, &kh) &&
+      (!mx && gemm_h_ok<L_KR, L_KR>(c, c->h1, c->ldAH1, c->dz2, c->ldAH2, c->AH1, c->AH2, B, 0, &kh) &&
        gemm_h_ok<L_RK, L_RK>(c, c->dz2, c->ldAH2, P(c, c->theta, L.a[AW2]), c->AH2, B, c->AH1,
                              c->AH2, 1, &kh))
           ? act_twin(c, c->dz2)
@@ -751,8 +754,19 @@ static void actor_train_dev(ddpg_ctx* c, int B, bool fused, bool par = false) {
   e.out = c->slab_W2;
   e.ldo = c->AH2;
   e.out_split_stride = (long long)c->AH1 * c->AH2;
-  GemmPlan pW2 = gemm_launch<L_KR, L_KR>(c, "wgrad", c->h1, c->ldAH1, c->dz2, c->ldAH2, c->AH1,
-                                         c->AH2, B, e, 0, c->split_cap_W2, G + L.a[AW2].off);
+  GemmPlan pW2;
+  if (mx) {  // dW2^T and dh1 in one go
+    ProfScope ps(c, "mx_grad", 4.0 * B * c->AH1 * c->AH2, 0);
+    mx_layer_grad_f32(c->cur, c->dz2, c->ldAH2, B, c->AH2, c->AH1, c->mx.xq, c->mx.w2_train,
+                      c->mx.dh1, c->mx.dw, c->mx.ws);
+    hipLaunchKernelGGL(sb_transpose_kernel, dim3(256), dim3(256), 0, c->cur, c->mx.dw, c->AH2,
+                       c->AH1, G + L.a[AW2].off);
+    HIP_TRY(hipGetLastError());
+    pW2.direct = true;
+  } else {
+    pW2 = gemm_launch<L_KR, L_KR>(c, "wgrad", c->h1, c->ldAH1, c->dz2, c->ldAH2, c->AH1, c->AH2, B,
+                                  e, 0, c->split_cap_W2, G + L.a[AW2].off);
+  }
   const long long nW2 = (long long)c->AH1 * c->AH2;
   if (c->comm) {
     // data parallel: dW2 (the bulk of the actor's gradient) reduced and its
@@ -779,15 +793,28 @@ static void actor_train_dev(ddpg_ctx* c, int B, bool fused, bool par = false) {
   e.colsum = colpart1;
   e.ld_colsum = c->AH1;
   const float* w2p = P(c, c->theta, L.a[AW2]);
-  const bool f1 = nw_ok(c, c->dz2, c->ldAH2, w2p, c->AH2, B, c->AH1, c->AH2, c->s, c->ldS, c->S,
+  const bool f1 = !mx && nw_ok(c, c->dz2, c->ldAH2, w2p, c->AH2, B, c->AH1, c->AH2, c->s, c->ldS, c->S,
                         c->nw_W1);
   if (f1) {
     nw_set(e, 0, c->s, c->ldS, c->S, c->nw_W1, c->AH1);
     e.out = nullptr;
     e.outh = nullptr;
   }
-  GemmPlan pz1 = gemm_launch<L_RK, L_RK>(c, "dx", c->dz2, c->ldAH2, w2p, c->AH2, B, c->AH1,
-                                         c->AH2, e);
+  GemmPlan pz1;
+  if (mx) {
+    pz1.bm = 64;
+    hipLaunchKernelGGL(elu_grad_kernel, dim3(ceil_div(c->AH1, 64), ceil_div(B, 64)), dim3(256), 0,
+                       c->cur, c->mx.dh1, c->AH1, c->mx.h1, c->ldAH1, B, c->AH1, c->dz1, c->ldAH1,
+                       colpart1);
+    HIP_TRY(hipGetLastError());
+    const Twin t = act_twin(c, c->dz1);  // what dW1's product reads
+    if (t.p)
+      hipLaunchKernelGGL(twin_kernel, dim3(std::min(ceil_div(B * c->ldAH1, 256), 2048)), dim3(256), 0,
+                         c->cur, c->dz1, (long long)B * c->ldAH1, t.p, t.ps, c->hnp);
+    HIP_TRY(hipGetLastError());
+  } else {
+    pz1 = gemm_launch<L_RK, L_RK>(c, "dx", c->dz2, c->ldAH2, w2p, c->AH2, B, c->AH1, c->AH2, e);
+  }
   // dW1 = s^T . dz1  (unless fused above)
   GemmPlan pW1;
   if (!f1)
@@ -1487,6 +1514,106 @@ int ddpg_soft_update(ddpg_ctx* c, int mask) {
   return guard(c, [&] {
     twins_refresh(c);
     soft_update_dev(c, mask, 0);
+    HIP_TRY(hipStreamSynchronize(c->stream));
+  });
+}
+
+// ---------------------------------------------------------------- 4-bit policy
+// The actor with its hidden layer (networks.py:57-58, all but a few percent of
+// its weights) in MXFP4: h1 is quantised, multiplied with the quantised W2 and
+// accumulated in fp32; the first layer reads the raw state and the output layer
+// makes the action, both in the context's precision.
+static void mx_alloc(ddpg_ctx* c, bool train) {
+  auto& m = c->mx;
+  auto get = [](auto*& p, size_t bytes) {
+    if (p) return;
+    void* q = nullptr;
+    HIP_TRY(hipMalloc(&q, std::max<size_t>(bytes, 16)));
+    HIP_TRY(hipMemset(q, 0, bytes));
+    p = static_cast<std::remove_reference_t<decltype(p)>>(q);
+  };
+  const size_t B = c->Bmax;
+  get(m.xq, mx_bytes(c->Bmax, c->AH1));
+  get(m.h1, B * c->ldAH1 * 4);
+  get(m.h2, B * c->ldAH2 * 4);
+  get(m.snap, (c->L.actor_end - c->L.actor_begin) * 4);
+  get(m.w2, mx_bytes(c->AH2, c->AH1));
+  if (train) {
+    get(m.w2_train, mx_bytes(c->AH2, c->AH1));
+    get(m.dh1, B * c->AH1 * 4);
+    get(m.dw, (size_t)c->AH2 * c->AH1 * 4);
+    // the largest of all batches' (a plan goes by the batch in 32s)
+    size_t ws = 0;
+    for (int b = 32; b < c->Bmax + 32; b += 32)
+      ws = std::max(ws, mx_layer_grad_ws(b, c->AH2, c->AH1));
+    get(m.ws, ws);
+  }
+  HIP_TRY(hipDeviceSynchronize());
+}
+
+// base: the actor's flat region; w2: its hidden layer, quantised
+static void mx_actor_fwd(ddpg_ctx* c, const float* base, const uint8_t* w2, int B, float* h2,
+                         float* o, bool keep) {
+  const Layout& L = c->L;
+  const TkPart tp = actor_l1_part(c, base, c->s, B, c->mx.h1, nullptr);
+  if (!thin_k_launch(c, "fwd", &tp, 1, B)) {
+    GemmEpi e = epi_none();
+    e.out = c->mx.h1;
+    e.ldo = c->ldAH1;
+    e.bias = P(c, base, L.a[AB1]);
+    e.act = 1;
+    gemm_launch<L_RK, L_KR>(c, "fwd", c->s, c->ldS, P(c, base, L.a[AW1]), c->AH1, B, c->AH1, c->S,
+                            e);
+  }
+  {
+    ProfScope ps(c, "mx_fwd", 2.0 * B * c->AH1 * c->AH2, 0);
+    mx_layer_f32(c->cur, c->mx.h1, c->ldAH1, B, c->AH1, w2, c->AH2, P(c, base, L.a[AB2]),
+                 DDPG_ACT_ELU, h2, c->ldAH2, c->mx.xq, keep);
+  }
+  hipLaunchKernelGGL(project_kernel, dim3(ceil_div(B, 4)), dim3(256), 0, c->cur, h2, c->ldAH2,
+                     c->AH2, P(c, base, L.a[AW3]), c->A, B, c->ppart);
+  HIP_TRY(hipGetLastError());
+  actor_out_launch(c, 1, B, o, c->mu);
+}
+
+int ddpg_actor_publish_mx(ddpg_ctx* c, int target) {
+  return guard(c, [&] {
+    mx_alloc(c, false);
+    const float* base = target ? c->target : c->theta;
+    HIP_TRY(hipMemcpyAsync(c->mx.snap, base, (c->L.actor_end - c->L.actor_begin) * 4,
+                           hipMemcpyDeviceToDevice, c->stream));
+    mx_quantize_f32(c->stream, P(c, c->mx.snap, c->L.a[AW2]), c->AH2, c->AH1, 1, c->AH2, c->mx.w2);
+    c->mx.published = true;
+  });
+}
+
+int ddpg_actor_forward_mx(ddpg_ctx* c, const float* s, int B, float* a_out) {
+  return guard(c, [&] {
+    check_b(c, B);
+    if (!c->mx.published)
+      throw DdpgError(DDPG_ESTATE, "no 4-bit policy was published (ddpg_actor_publish_mx)");
+    upload_rows(c, c->s, c->ldS, s, B, c->S);
+    mx_actor_fwd(c, c->mx.snap, c->mx.w2, B, c->mx.h2, nullptr, false);
+    download_rows(c, a_out, c->mu, c->ldA, B, c->A);
+  });
+}
+
+int ddpg_actor_train_mx(ddpg_ctx* c, const float* s, const float* a_gradient, int B) {
+  return guard(c, [&] {
+    check_b(c, B);
+    mx_alloc(c, true);
+    twins_refresh(c);
+    upload_rows(c, c->s, c->ldS, s, B, c->S);
+    HIP_TRY(hipMemcpyAsync(c->dain, a_gradient, (size_t)B * c->A * 4, hipMemcpyHostToDevice,
+                           c->stream));
+    mx_quantize_f32(c->stream, P(c, c->theta, c->L.a[AW2]), c->AH2, c->AH1, 1, c->AH2,
+                    c->mx.w2_train);
+    mx_actor_fwd(c, c->theta, c->mx.w2_train, B, c->h2, c->o, true);
+    hipLaunchKernelGGL(action_grad_kernel, dim3(ceil_div(B * c->A, 256)), dim3(256), 0, c->stream,
+                       c->dain, 1, B, c->A, B, c->o, c->ldA, c->cfg.action_scale, nullptr,
+                       c->dz3);
+    HIP_TRY(hipGetLastError());
+    actor_train_dev(c, B, false, false, true);
     HIP_TRY(hipStreamSynchronize(c->stream));
   });
 }

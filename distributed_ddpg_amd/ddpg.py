@@ -182,7 +182,10 @@ def run_worker(opt, task_index, env_name, episodes, device):
     while True:
         # exploration offset 1/(1 + global_step): global_step is the episode
         # counter restored from the checkpoint (ddpg.py:69, 250)
-        a = actor.predict(np.reshape(state, (1, S))) + (1.0 / (1.0 + global_step))
+        if opt.act_mx and t == 0:
+            actor.publish_mx()
+        act = actor.predict_mx if opt.act_mx else actor.predict
+        a = act(np.reshape(state, (1, S))) + (1.0 / (1.0 + global_step))
         state2, r, done, _ = env.step(a[0])
         replay.add(np.reshape(state, (S,)), np.reshape(a, (A,)), r, done,
                    np.reshape(state2, (S,)))

@@ -297,6 +297,28 @@ class ActorNetwork:
     def predict_target(self, inputs):
         return self._forward(inputs, True)
 
+    # --- the 4-bit policy (not in the reference): the hidden layer in MXFP4
+    def publish_mx(self, target=False):
+        """Snapshot the online (or target) actor as the 4-bit policy that
+        predict_mx acts on until the next call."""
+        check(lib.ddpg_actor_publish_mx(self.sess.ctx, int(target)), self.sess.ctx)
+
+    def predict_mx(self, inputs):
+        """predict() on the published 4-bit policy."""
+        ss = self.sess
+        s = ss._rows(self.preprocess_input(inputs), self.s_dim, any_batch=True)
+        fn = lambda x, n, o: check(lib.ddpg_actor_forward_mx(ss.ctx, fptr(x[0]), n, fptr(o)),
+                                   ss.ctx)
+        return ss._rowwise(fn, [s], self.a_dim)
+
+    def train_mx(self, inputs, a_gradient):
+        """train() through the 4-bit hidden layer (straight-through): the fp32
+        parameters learn to act well once quantised."""
+        ss = self.sess
+        s = ss._rows(self.preprocess_input(inputs), self.s_dim)
+        g = f32(a_gradient).reshape(s.shape[0], self.a_dim)
+        check(lib.ddpg_actor_train_mx(ss.ctx, fptr(s), fptr(g), s.shape[0]), ss.ctx)
+
     def update_target_network(self):
         check(lib.ddpg_soft_update(self.sess.ctx, _lib.SOFT_ACTOR), self.sess.ctx)
 

@@ -36,4 +36,5 @@ class Parameters:
         # MI355X build additions (not in the reference)
         self.hidden = (128, 200)        # networks.py:54-55,151-156
         self.grad_clip = None           # largest gradient norm (a number or (actor, critic))
+        self.act_mx = False             # act on the 4-bit policy, published every episode
         self.device = 0

@@ -139,6 +139,17 @@ int ddpg_critic_action_grad(ddpg_ctx* ctx, const float* s, const float* a, int B
 int ddpg_actor_train(ddpg_ctx* ctx, const float* s, const float* a_gradient, int B);
 /* update_target_network (mask: DDPG_SOFT_*)        networks.py:34-37,87-88,126-128,195-196 */
 int ddpg_soft_update(ddpg_ctx* ctx, int mask);
+/* The 4-bit policy: the actor with its hidden layer (W2, all but a few percent of
+ * its weights) in MXFP4, for workers that act on a published copy.  publish_mx
+ * takes a snapshot of the online (target = 0) or target actor; forward_mx is
+ * ddpg_actor_forward on that snapshot (DDPG_ESTATE before the first), whatever was
+ * trained since.  train_mx is ddpg_actor_train through the 4-bit hidden layer:
+ * the forward quantises h1 and W2, the gradient passes straight through the
+ * quantisation to the fp32 W2 and h1, and Adam (with ddpg_set_grad_clip's clip)
+ * updates the fp32 parameters.  B in [1, batch_max]. */
+int ddpg_actor_publish_mx(ddpg_ctx* ctx, int target);
+int ddpg_actor_forward_mx(ddpg_ctx* ctx, const float* s, int B, float* a_out);
+int ddpg_actor_train_mx(ddpg_ctx* ctx, const float* s, const float* a_gradient, int B);
 /* per-feature affine input scaler (sklearn StandardScaler.transform, ddpg.py:184-189,
  * networks.py:65-69,164-168): (x - mean) / scale in float64, then one rounding to
  * fp32.  Applied ONLY where the library reads raw replay rows (the fused
