@@ -103,16 +103,16 @@ DDPG_DEV void mx_store_tile(const MxOut& o, lds_char* strip, int i0, int j0,
   typedef __attribute__((address_space(3))) tx4 lds_tx4;
   typedef __attribute__((address_space(3))) u32x4 lds_u4;
   const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int i = 0; i < TI; ++i) {
+  static_for<TI>([&](auto i_c) {
+    constexpr int i = decltype(i_c)::value;
     lds_char* const s = strip + (i & 1) * 16 * ROW;
-#pragma unroll
-    for (int j = 0; j < TJ; ++j) {
+    static_for<TJ>([&](auto j_c) {
+      constexpr int j = decltype(j_c)::value;
       tx4 v;
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = (T)mx_act(__fadd_rn(acc[i][j][r], bias[j][r]), o.act);
       *(lds_tx4*)(s + (lane & 15) * ROW + (j * 16 + (lane >> 4) * 4) * (int)sizeof(T)) = v;
-    }
+    });
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int u = lane; u < 16 * PER; u += 64) {
@@ -133,7 +133,7 @@ DDPG_DEV void mx_store_tile(const MxOut& o, lds_char* strip, int i0, int j0,
       }
     }
     __builtin_amdgcn_wave_barrier();
-  }
+  });
 }
 
 // acc[j + r][i] += J fragment x I fragment, with scale bytes BJ of sj, BI of si
@@ -302,6 +302,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
   int jk = pt.k0 % max(g.kt, 1);  // J's depth step of the next load (I's planes go on, J's repeat)
 
   // this wave's pieces of a step: source of the next step to load, LDS place.
+  // The sources are the same for all lanes (scalar registers, scalar adds), a
+  // lane's place in a piece is its own.
   // Row groups past the operand's last are read from the last one's place
   // (their results are not stored).
   const uint8_t* src[C::PW];
@@ -314,8 +316,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
     const int grp = isj[p] ? min(tj * C::GJ + f - C::GI, g.J.groups - 1)
                            : min(ti * C::GI + f, g.I.groups - 1);
     src[p] = (isj[p] ? g.J.p + ((size_t)grp * g.kt + jk) * 1024
-                     : g.I.p + ((size_t)grp * g.kt * g.planes + pt.k0) * 1024) +
-             lane * 16;
+                     : g.I.p + ((size_t)grp * g.kt * g.planes + pt.k0) * 1024);
   }
 #pragma unroll
   for (int p = 0; p < C::SW; ++p) {
@@ -323,18 +324,19 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
     const bool j = f >= C::GI / 4;
     const int grp = j ? min(tj * (C::GJ / 4) + f - C::GI / 4, g.J.groups / 4 - 1)
                       : min(ti * (C::GI / 4) + f, g.I.groups / 4 - 1);
-    ssrc[p] = (j ? g.J.scales : g.I.scales) + ((size_t)grp * g.kt + pt.k0) * 256 + lane * 4;
+    ssrc[p] = (j ? g.J.scales : g.I.scales) + ((size_t)grp * g.kt + pt.k0) * 256;
   }
   lds_char* const base = (lds_char*)smem;
+  const unsigned l16 = lane * 16, l4 = lane * 4;
   auto load_piece = [&](int slot, auto p_c) {
     constexpr int p = decltype(p_c)::value;
     if constexpr (p < C::PW) {
-      lds_load16(src[p], base + slot * C::SLOT + (wave * C::PW + p) * 1024);
+      lds_load16(src[p] + l16, base + slot * C::SLOT + (wave * C::PW + p) * 1024);
       src[p] += 1024;
       if (!FP4 && isj[p] && jk + 1 == g.kt) src[p] -= (size_t)g.kt * 1024;
     } else {
       constexpr int q = p - C::PW;
-      lds_load4(ssrc[q],
+      lds_load4(ssrc[q] + l4,
                 base + slot * C::SLOT + (C::GI + C::GJ) * 1024 + (wave * C::SW + q) * 256);
       ssrc[q] += 256;
     }
@@ -345,10 +347,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
   static_assert(NM >= TJ + 1 + G && NM >= 2 * TJ, "gaps for the loads and the reads");
 
   f32x4 acc[TI][TJ];
-#pragma unroll
-  for (int i = 0; i < TI; ++i)
-#pragma unroll
-    for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  static_for<TI * TJ>([&](auto q) {
+    acc[decltype(q)::value / TJ][decltype(q)::value % TJ] = f32x4{0.f, 0.f, 0.f, 0.f};
+  });
 
   if (nk > 0) {
     u32x4 fi[TI], fl[2], fj[2][TJ];  // fi[TI - 1] is fl
