@@ -387,3 +387,72 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i, (n, y) in enumerate(got):
         assert torch.equal(n, want[i % 4][0]) and torch.equal(y, want[i % 4][1])
+
+
+# ---------------------------------------------------------------- large
+def dev64(t):
+    return t.double().cuda()
+
+
+@pytest.mark.parametrize("dt,act", [("fp32", "elu"), ("bf16", None), ("fp16", "tanh")])
+@pytest.mark.parametrize("M,K,N", [(1025, 300, 1100),   # 64 x 64 tiles
+                                   (2001, 300, 1703),   # 128 x 128
+                                   (2500, 2049, 1600),
+                                   (4001, 200, 4099),   # 256 x 256
+                                   (4096, 1100, 4352)])
+def test_linear_tiles(M, K, N, dt, act):
+    x, w, b = rnd(M, K, dt=dt, seed=1), rnd(N, K, seed=2, scale=K ** -0.5), rnd(N, seed=3)
+    xv, wv = dev64(O.mx_values(x)), dev64(O.mx_values(w))
+    want = O.act(xv @ wv.T + dev64(b), act)
+    s = xv.abs() @ wv.abs().T + dev64(b).abs()
+    y = ops.mx_linear(x.cuda(), ops.mx_quantize(w.cuda()), b.cuda(), act)
+    assert y.dtype == DT[dt]
+    err = (y.double() - want).abs()
+    assert (err <= linear_tol(want, s, K, DT[dt], 1.0 if act else 0.0)).all(), float(err.max())
+
+
+@pytest.mark.parametrize("M,K,N,dt", [(1100, 900, 1050, "fp16"),   # 64 x 64 tiles
+                                      (2050, 2049, 2047, "bf16"),  # 128 x 128
+                                      (8192, 4096, 64, "bf16"),    # and dW in 11 splits
+                                      (8190, 65, 4095, "fp32"),    # 256 x 256, 4 and 8 splits
+                                      (4099, 2051, 2040, "fp32"),
+                                      (8000, 17, 5, "fp32")])      # 32 x 32, dW in 12 splits
+def test_linear_grad_tiles(M, K, N, dt):
+    x, w, dy = rnd(M, K, seed=1), rnd(N, K, seed=2), rnd(M, N, dt=dt, seed=3)
+    xv, wv, d = dev64(O.mx_values(x)), dev64(O.mx_values(w)), dev64(dy)
+    want = (d @ wv, d.T @ xv, d.sum(0))
+    s = (d.abs() @ wv.abs(), d.abs().T @ xv.abs(), d.abs().sum(0))
+    xq, wq, dyd = ops.mx_quantize(x.cuda()), ops.mx_quantize(w.cuda()), dy.cuda()
+    got = ops.mx_linear_grad(dyd, xq, wq)
+    for g, v, a, k, t in zip(got, want, s, (N, M, M), (dy.dtype, torch.float32, torch.float32)):
+        err = (g.double() - v).abs()
+        assert (err <= a * (3 * k + 2) * 2.0 ** -23 + half_step(t, v)).all(), float(err.max())
+    for _ in range(3):  # whichever split comes last
+        assert all(torch.equal(a, b) for a, b in zip(ops.mx_linear_grad(dyd, xq, wq), got))
+    dx, _, _ = ops.mx_linear_grad(dyd, xq, wq, need=(True, False), bias=False)
+    _, dw, _ = ops.mx_linear_grad(dyd, xq, wq, need=(False, True), bias=False)
+    assert torch.equal(dx, got[0]) and torch.equal(dw, got[1])
+
+
+def test_offsets_past_32_bits():
+    big = torch.empty((1 << 32) + 4096, dtype=torch.bfloat16, device="cuda")
+    x = rnd(17, 200, dt="bf16", seed=8)
+    far = big.as_strided((17, 200), (1 << 28, 1))
+    far.copy_(x.cuda())
+    same(ops.mx_quantize(far).dequantize(), O.mx_values(x))
+    wq = ops.mx_quantize(rnd(40, 200).cuda())
+    assert torch.equal(ops.mx_linear(far, wq), ops.mx_linear(x.cuda(), wq))
+    turned = big.as_strided((200, 17), (1, 1 << 28))
+    same(ops.mx_quantize(turned).dequantize(), O.mx_values(x.t()))
+    assert float(ops.global_norm([far])) == float(ops.global_norm([x.cuda()]))
+    dy = big.as_strided((17, 40), (1 << 28, 1))
+    dy.copy_(x[:, :40].cuda())
+    xq = ops.mx_quantize(x.cuda())
+    a = ops.mx_linear_grad(dy, xq, wq)
+    b = ops.mx_linear_grad(x[:, :40].cuda(), xq, wq)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    big.zero_()
+    big[0], big[1 << 31], big[-1] = 2.0, 3.0, 6.0
+    assert float(ops.global_norm([big])) == 7.0
+    ops.clip_by_global_norm([big], 3.5, inplace=True)
+    assert [float(big[i]) for i in (0, 1 << 31, -1)] == [1.0, 1.5, 3.0]

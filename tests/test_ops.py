@@ -65,6 +65,8 @@ def test_norm_entry_refusals():
     twice = arr(ctypes.c_void_p, 4096, 4096)
     refused(clip(1.0, 2, twice, twice, two), "tensors 0 and 1 overlap")
     refused(clip(1.0, 1, p, p, one, arr(ctypes.c_int64, 4), arr(ctypes.c_int64, 3)), "itself")
+    refused(L.ddpg_clip_by_global_norm(0, None, 1, f32, p, p, one, None, None, 1.0, 4100, None, 0,
+                                       None), "use_norm lies in tensor 0")
     # two column ranges of rows 10 apart that share column 3
     cols, ld = arr(ctypes.c_int64, 4, 4), arr(ctypes.c_int64, 10, 10)
     at = arr(ctypes.c_void_p, 4096, 4096 + 3 * 4)
