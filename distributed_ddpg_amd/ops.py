@@ -127,7 +127,7 @@ class _List:
         self.ws_bytes = lib.ddpg_global_norm_workspace(self.n)
 
     def empty(self, n, dtype):
-        return torch.empty(n, dtype=dtype, device=self.kept[0].device)
+        return self.kept[0].new_empty(n, dtype=dtype)
 
 
 def global_norm(t_list):
@@ -182,13 +182,17 @@ class MXTensor:
     them along a row, in the order the matrix instructions read (an opaque buffer;
     .dequantize() gives the values).  17/32 byte a value."""
 
-    __slots__ = ("buffer", "shape", "device", "_index", "_codes", "_scales")
+    __slots__ = ("buffer", "shape", "_index", "_codes", "_scales")
 
     def __init__(self, buffer, shape):
         self.buffer, self.shape = buffer, shape
-        self.device, self._index = buffer.device, buffer.get_device()
+        self._index = buffer.get_device()
         self._codes = buffer.data_ptr()  # the scales come behind the codes
         self._scales = self._codes + buffer.numel() // 17 * 16
+
+    @property
+    def device(self):
+        return self.buffer.device
 
     def dequantize(self, dtype=torch.float32):
         return mx_dequantize(self, dtype)
@@ -228,8 +232,7 @@ def mx_quantize(x):
     NaN as a whole."""
     code = _matrix("x", x)
     (rows, cols), (s0, s1) = x.shape, x.stride()
-    q = MXTensor(torch.empty(_mx_bytes(rows, cols), dtype=torch.uint8, device=x.device),
-                 (rows, cols))
+    q = MXTensor(x.new_empty(_mx_bytes(rows, cols), dtype=torch.uint8), (rows, cols))
     _check(lib.ddpg_mx_quantize(q._index, _stream(q._index), code, x.data_ptr(), rows, cols, s0,
                                 s1, q._codes, q._scales))
     return q
@@ -241,7 +244,7 @@ def mx_dequantize(q, dtype=torch.float32):
     _mx("q", q)
     if dtype not in _DTYPES:
         raise ValueError("dtype: %s is none of float32, bfloat16, float16" % dtype)
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    out = q.buffer.new_empty(q.shape, dtype=dtype)
     _check(lib.ddpg_mx_dequantize(q._index, _stream(q._index), q._codes, q._scales, q.shape[0],
                                   q.shape[1], _DTYPES[dtype], out.data_ptr(), q.shape[1]))
     return out
@@ -272,7 +275,7 @@ def mx_linear(x, w, bias=None, act=None, dtype=None):
         codes = scales = None
         nb = lib.ddpg_mx_linear_workspace(M, K, N)
         if nb:
-            ws = torch.empty(nb, dtype=torch.uint8, device=w.device)
+            ws = w.buffer.new_empty(nb)
             wp = ws.data_ptr()
         dtype = dtype or x.dtype
     yc = _DTYPES.get(dtype)
@@ -286,7 +289,7 @@ def mx_linear(x, w, bias=None, act=None, dtype=None):
                 N, w.device, tuple(bias.shape), bias.device))
         bias = bias.contiguous()
         bp = bias.data_ptr()
-    y = torch.empty((M, N), dtype=dtype, device=w.device)
+    y = w.buffer.new_empty((M, N), dtype=dtype)
     _check(lib.ddpg_mx_linear(index, _stream(index), xc, xp, s0, s1, codes, scales, M, K, w._codes,
                               w._scales, N, bc, bp, _ACTS[act], yc, y.data_ptr(), N, wp,
                               nb))
@@ -301,7 +304,7 @@ def mx_linear_grad(dy, x, w, need=(True, True), bias=True):
     are the gradients of the matrices that were quantised.  need: whether dx,
     dw are wanted (None otherwise); bias: whether db is."""
     code = _matrix("dy", dy)
-    index, dev = dy.get_device(), dy.device
+    index = dy.get_device()
     _mx("x", x, None, index)
     _mx("w", w, x.shape[1], index)
     (M, K), N = x.shape, w.shape[0]
@@ -309,17 +312,17 @@ def mx_linear_grad(dy, x, w, need=(True, True), bias=True):
         raise ValueError("dy: expected [%d, %d], got %s" % (M, N, tuple(dy.shape)))
     dx = dw = db = pdx = pdw = pdb = None
     if need[0]:
-        dx = torch.empty((M, K), dtype=dy.dtype, device=dev)
+        dx = dy.new_empty((M, K))
         pdx = dx.data_ptr()
     if need[1]:
-        dw = torch.empty((N, K), dtype=torch.float32, device=dev)
+        dw = dy.new_empty((N, K), dtype=torch.float32)
         pdw = dw.data_ptr()
     if bias:
-        db = torch.empty(N, dtype=torch.float32, device=dev)
+        db = dy.new_empty(N, dtype=torch.float32)
         pdb = db.data_ptr()
     nb = lib.ddpg_mx_linear_grad_workspace(code, M, N, K, dx is not None, dw is not None,
                                            db is not None)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    ws = x.buffer.new_empty(nb)
     s0, s1 = dy.stride()
     _check(lib.ddpg_mx_linear_grad(index, _stream(index), code, dy.data_ptr(), s0, s1, M, N, K,
                                    x._codes, x._scales, w._codes, w._scales, pdx, pdw, pdb,
