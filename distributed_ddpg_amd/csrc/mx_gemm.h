@@ -88,48 +88,62 @@ DDPG_DEV void mx_bias(const MxOut& o, int j, float* b) {
     b[r] = o.bias && j + r < o.J ? load_elem(o.bias, o.bias_dtype, j + r) : 0.f;
 }
 
-// A wave's TI x TJ fragments to the output by whole rows: 16 rows at a time go
-// through a strip of LDS of its own (two in turn), from where 8 (bf16, fp16) or
-// 16 (fp32) lanes write a row's 64 outputs as 16-byte stores.  Straight from the
-// registers a store covers 32 bytes of a row, and the write-out cost 28 us a
-// 256 x 256 tile.
-template <int DT, int TI, int TJ>
+// A wave's TI x 4 fragments to the output by whole rows: 64 rows at a time go
+// through 16 KiB of LDS of its own as the fp32 sums (16-byte units of a row
+// swizzled by the row, free of bank conflicts), from where 8 lanes take a row's 64
+// outputs, 8 each: bias, activation, one rounding, 16-byte stores.  Straight from
+// the registers a store covers 32 bytes of a row (28 us a 256 x 256 tile).  The
+// second half is a loop, not unrolled code: with the activations inlined at every
+// fragment the code outgrew the instruction cache (fp4 8192 x 4096 x 4096 between other
+// kernels: 92 us so, 75 as a loop).
+template <int DT, int TI>
 DDPG_DEV void mx_store_tile(const MxOut& o, lds_char* strip, int i0, int j0,
-                            const f32x4 (&acc)[TI][TJ], const float (&bias)[TJ][4]) {
+                            const f32x4 (&acc)[TI][4]) {
   typedef typename Elem<DT>::type T;
-  constexpr int ROW = TJ * 16 * sizeof(T) + 16;  // padded: rows start 4 banks apart
-  constexpr int V = 16 / sizeof(T), PER = TJ * 16 / V;  // 16-byte units of a row
-  typedef T tx4 __attribute__((ext_vector_type(4)));
-  typedef __attribute__((address_space(3))) tx4 lds_tx4;
-  typedef __attribute__((address_space(3))) u32x4 lds_u4;
-  const int lane = threadIdx.x & 63;
-  static_for<TI>([&](auto i_c) {
-    constexpr int i = decltype(i_c)::value;
-    lds_char* const s = strip + (i & 1) * 16 * ROW;
-    static_for<TJ>([&](auto j_c) {
-      constexpr int j = decltype(j_c)::value;
-      tx4 v;
+  constexpr int V = Elem<DT>::V;
+  typedef __attribute__((address_space(3))) f32x4 lds_v4f;
+  const int lane = threadIdx.x & 63, q = lane & 7, col = j0 + 8 * q;
+  auto at = [&](int r, int unit) { return (lds_v4f*)(strip + r * 256 + ((unit ^ r) & 15) * 16); };
+  float b[8];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = (T)mx_act(__fadd_rn(acc[i][j][r], bias[j][r]), o.act);
-      *(lds_tx4*)(s + (lane & 15) * ROW + (j * 16 + (lane >> 4) * 4) * (int)sizeof(T)) = v;
+  for (int k = 0; k < 8; ++k)
+    b[k] = o.bias && col + k < o.J ? load_elem(o.bias, o.bias_dtype, col + k) : 0.f;
+  static_for<TI / 4>([&](auto h_c) {
+    constexpr int h = decltype(h_c)::value;
+    static_for<16>([&](auto f_c) {
+      constexpr int i = decltype(f_c)::value / 4, j = decltype(f_c)::value % 4;
+      *at(i * 16 + (lane & 15), j * 4 + (lane >> 4)) = acc[4 * h + i][j];
     });
     __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int it = 0; it < 8; ++it) {
+      const int r = it * 8 + (lane >> 3), row = i0 + h * 64 + r;
+      const f32x4 lo = *at(r, 2 * q), hi = *at(r, 2 * q + 1);
+      if (row >= o.I || col >= o.J) continue;
+      float v[8];
 #pragma unroll
-    for (int u = lane; u < 16 * PER; u += 64) {
-      const int r = u / PER, c = u % PER * V;
-      const u32x4 w = *(lds_u4*)(s + r * ROW + c * (int)sizeof(T));
-      const int row = i0 + i * 16 + r, col = j0 + c;
-      if (row < o.I && col < o.J) {
-        T* p = static_cast<T*>(o.y) + row * o.ldo + col;
-        if (o.vec && col + V <= o.J) {
-          *reinterpret_cast<u32x4*>(p) = w;
-        } else {
-          T e[V];
-          __builtin_memcpy(e, &w, 16);
+      for (int k = 0; k < 4; ++k) {
+        v[k] = __fadd_rn(lo[k], b[k]);
+        v[4 + k] = __fadd_rn(hi[k], b[4 + k]);
+      }
+      if (o.act == DDPG_ACT_ELU) {
 #pragma unroll
-          for (int k = 0; k < V; ++k)
-            if (col + k < o.J) p[k] = e[k];
+        for (int k = 0; k < 8; ++k) v[k] = elu_f(v[k]);
+      } else if (o.act == DDPG_ACT_TANH) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = tanhf(v[k]);
+      }
+      T* p = static_cast<T*>(o.y) + row * o.ldo + col;
+      if (o.vec && col + 8 <= o.J) {
+#pragma unroll
+        for (int k = 0; k < 8; k += V) {
+          const U16B u = Elem<DT>::pack(v + k);
+          *reinterpret_cast<u32x4*>(p + k) = u32x4{u.v[0], u.v[1], u.v[2], u.v[3]};
         }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (col + k < o.J) p[k] = (T)v[k];
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -271,6 +285,7 @@ struct RingCfg {
   static constexpr int SLOT = (GI + GJ) * 1024 + SP * 256;
   static constexpr int LDS = NS * SLOT;
   static_assert(PW * NW == GI + GJ && SW * NW == SP && TI % 4 == 0 && TJ % 4 == 0, "whole pieces");
+  static_assert(TJ == 4 && LDS >= NW * 16384, "mx_store_tile");
   static_assert(LDS <= 160 * 1024, "LDS");
   static_assert((GI + GJ) * 1024 + SP * 256 < 65536, "LDS offsets are immediates");
 };
@@ -453,14 +468,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
   if (!FP4 && g.splits > 1 && !mx_join<TI * TJ>(g, pt, &acc[0][0], threadIdx.x, C::NT, true))
     return;
   __syncthreads();  // the ring is done with: it carries the results out
-  float bias[TJ][4];
-#pragma unroll
-  for (int j = 0; j < TJ; ++j)
-    mx_bias(g.o, (tj * C::GJ + wj * TJ + j) * 16 + (lane >> 4) * 4, bias[j]);
   by_dtype(g.o.dtype, [&](auto dt) {
-    mx_store_tile<decltype(dt)::value, TI, TJ>(g.o, base + wave * (C::LDS / C::NW / 1024 * 1024),
-                                               (ti * C::GI + wi * TI) * 16,
-                                               (tj * C::GJ + wj * TJ) * 16, acc, bias);
+    mx_store_tile<decltype(dt)::value, TI>(g.o, base + wave * 16384, (ti * C::GI + wi * TI) * 16,
+                                           (tj * C::GJ + wj * TJ) * 16, acc);
   });
 }
 
