@@ -202,7 +202,7 @@ DDPG_DEV void mx_turn(const MxMat& q, uint8_t* __restrict__ out, int b, __bf16 (
 // the other): flat, rows m and depth n; turned, rows n and depth m; both depths
 // to whole 64s, the padding 0.  And the tile's column sums.
 template <int DT, int P>
-DDPG_DEV void mx_dy(const MxPrep& a, int b, float (&t)[64][65]) {
+DDPG_DEV void mx_dy(const MxPrep& a, int b, float (&t)[64][65], float (&red)[4][64]) {
   const typename Elem<DT>::type* dy = static_cast<const typename Elem<DT>::type*>(a.dy);
   const int M = a.M, N = a.N, nn = (N + 63) >> 6, mb = b / nn, nb = b % nn;
   const int m0 = mb * 64, n0 = nb * 64, nm = (M + 63) >> 6;
@@ -212,11 +212,18 @@ DDPG_DEV void mx_dy(const MxPrep& a, int b, float (&t)[64][65]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       v[i] = (float)dy[min(m0 + w + 4 * i, M - 1) * a.sr + min(n0 + l, N - 1) * a.sc];
+    float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      t[w + 4 * i][l] = m0 + w + 4 * i < M && n0 + l < N ? v[i] : 0.f;
+    for (int i = 0; i < 16; ++i) {
+      const float x = m0 + w + 4 * i < M && n0 + l < N ? v[i] : 0.f;
+      t[w + 4 * i][l] = x;
+      s += x;
+    }
+    red[w][l] = s;
   }
   __syncthreads();
+  if (a.part && w == 0 && n0 + l < N)
+    a.part[(size_t)mb * N + n0 + l] = ((red[0][l] + red[1][l]) + red[2][l]) + red[3][l];
   // 4 row groups x 2 depth steps: a wave takes row group w
   auto put = [&](uint8_t* out, int grp, int steps, int s0, auto at) {
 #pragma unroll
@@ -237,25 +244,21 @@ DDPG_DEV void mx_dy(const MxPrep& a, int b, float (&t)[64][65]) {
   };
   if (a.flat) put(a.flat, mb * 4 + w, nn * 2, nb * 2, [&](int r, int c) { return t[r][c]; });
   if (a.turned) put(a.turned, nb * 4 + w, nm * 2, mb * 2, [&](int r, int c) { return t[c][r]; });
-  if (a.part && w == 0 && n0 + l < N) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 64; ++i) s += t[i][l];
-    a.part[(size_t)mb * N + n0 + l] = s;
-  }
 }
 
 template <int DT>
 __global__ __launch_bounds__(256) void mx_prep_kernel(MxPrep a) {
   __shared__ __attribute__((aligned(16))) union {
     __bf16 turn[128][72];
-    float dy[64][65];
+    struct {
+      float t[64][65], red[4][64];
+    } dy;
   } t;
   const int b = blockIdx.x;
   if (b == 0)
     for (int i = threadIdx.x; i < a.ntickets; i += 256) a.tickets[i] = 0;
   if (b < a.dy_blocks)
-    mx_dy<DT, mx_planes(DT)>(a, b, t.dy);
+    mx_dy<DT, mx_planes(DT)>(a, b, t.dy.t, t.dy.red);
   else if (b < a.dy_blocks + a.w_blocks)
     mx_turn(a.w, a.wt, b - a.dy_blocks, t.turn);
   else
@@ -299,10 +302,6 @@ void mx_quantize_launch(hipStream_t st, int dtype, const void* x, int rows, int 
   HIP_TRY(hipGetLastError());
 }
 
-static bool mx_rows_aligned(const MxOut& o) {
-  return o.ldo * elem_size(o.dtype) % 16 == 0 && aligned16(o.y);
-}
-
 // The kernels of a product: tiles of 256 x 256 and 128 x 128 through LDS, and 64 x 64
 // and 32 x 32 with the depth split over a block's 4 and 8 waves.
 enum { MX_256, MX_128, MX_64, MX_32 };
@@ -318,9 +317,8 @@ static void mx_gemm_launch(hipStream_t st, MxGemms& p, int pick) {
   auto launch = [&](auto k, int threads) {
     long long n = 0;
     for (int i = 0; i < 2; ++i) {
-      MxOut& o = p.g[i].o;
+      const MxOut& o = p.g[i].o;
       if (i < p.n) {
-        o.vec = mx_rows_aligned(o);
         n += mx_tiles(o.I, o.J, tile) * p.g[i].splits;
       }
       p.end[i] = (int)grid_x(n);
@@ -362,9 +360,8 @@ void mx_linear_launch(hipStream_t st, const MxMat& x, const MxMat& w, const MxOu
 // and 7.1, of 4096 10.2 and 7.8; 64 of 512 7.6 and 6.8 (and the launch's host time).
 static bool mx_rows_ok(int64_t M, int64_t K) { return M <= 64 && M * K <= 32768; }
 void mx_linear_rows_launch(hipStream_t st, int dtype, const void* x, long long sr, long long sc,
-                           int M, int K, const MxMat& w, MxOut o) {
+                           int M, int K, const MxMat& w, const MxOut& o) {
   if (!M || !o.J) return;
-  o.vec = mx_rows_aligned(o);
   const RawX r{x, sr, sc, M, K, sc == 1};
   by_dtype(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
@@ -471,7 +468,7 @@ void mx_linear_grad_launch(hipStream_t st, int dtype, const void* dy, long long 
                   {J, nullptr, ceil_div(K, 64) * 4},
                   steps,
                   L.P,
-                  {C, nullptr, K, ni, K, type, 0, DDPG_ACT_NONE, 0},
+                  {C, nullptr, K, ni, K, type, 0, DDPG_ACT_NONE},
                   L.splits[q],
                   reinterpret_cast<float*>(ws + L.slab[q]),
                   t};
@@ -500,7 +497,7 @@ void mx_quantize_f32(hipStream_t st, const float* x, int rows, int cols, long lo
 }
 void mx_layer_f32(hipStream_t st, const float* x, int ldx, int M, int K, const uint8_t* w, int N,
                   const float* bias, int act, float* y, int ldy, uint8_t* xq, bool keep) {
-  const MxOut o{y, bias, ldy, M, N, T_FP32, T_FP32, act, 0};
+  const MxOut o{y, bias, ldy, M, N, T_FP32, T_FP32, act};
   if (!keep && mx_rows_ok(M, K)) {
     mx_linear_rows_launch(st, T_FP32, x, ldx, 1, M, K, mx_in(w, N, K), o);
     return;
@@ -593,7 +590,7 @@ int ddpg_mx_linear(int device, void* stream, int x_dtype, const void* x, int64_t
     if (y_row_stride < N) throw einval("mx_linear: rows %lld apart overlap", (long long)y_row_stride);
     OnDevice on(device);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const MxOut o{y, bias, (long long)y_row_stride, (int)M, (int)N, dtype, bias_dtype, act, 0};
+    const MxOut o{y, bias, (long long)y_row_stride, (int)M, (int)N, dtype, bias_dtype, act};
     if (rows) {
       mx_linear_rows_launch(st, x_dtype, x, x_row_stride, x_col_stride, (int)M, (int)K, wq, o);
       return;

@@ -21,7 +21,6 @@ struct MxOut {
   const void* bias;
   long long ldo;
   int I, J, dtype, bias_dtype, act;
-  int vec;  // rows begin on 16-byte boundaries
 };
 
 struct FragOp {
@@ -51,10 +50,15 @@ struct MxGemms {
   int db_parts, db_n;
 };
 
-DDPG_DEV float mx_act(float v, int act) {
-  if (act == DDPG_ACT_ELU) return elu_f(v);
-  if (act == DDPG_ACT_TANH) return tanhf(v);
-  return v;
+template <int N>
+DDPG_DEV void mx_act(float (&v)[N], int act) {
+  if (act == DDPG_ACT_ELU) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = elu_f(v[k]);
+  } else if (act == DDPG_ACT_TANH) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = tanhf(v[k]);
+  }
 }
 
 // C[i][j .. j+3] of a lane to the output; b: the four biases
@@ -62,19 +66,16 @@ DDPG_DEV void mx_store(const MxOut& o, int i, int j, const f32x4& d, const float
   if (i >= o.I || j >= o.J) return;
   float v[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) v[r] = mx_act(__fadd_rn(d[r], b[r]), o.act);
+  for (int r = 0; r < 4; ++r) v[r] = __fadd_rn(d[r], b[r]);
+  mx_act(v, o.act);
   const long long at = i * o.ldo + j;
-  if (o.vec && j + 4 <= o.J) {
-    if (o.dtype == T_FP32) {
-      *reinterpret_cast<f32x4*>(static_cast<float*>(o.y) + at) = f32x4{v[0], v[1], v[2], v[3]};
-    } else if (o.dtype == T_BF16) {
-      const bf16x4 h = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-      *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(o.y) + at) = h;
-    } else {
-      typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-      const f16x4 h = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-      *reinterpret_cast<f16x4*>(static_cast<_Float16*>(o.y) + at) = h;
-    }
+  if (j + 4 <= o.J) {  // one store, whatever the row's alignment
+    by_dtype(o.dtype, [&](auto dt) {
+      typedef typename Elem<decltype(dt)::value>::type T;
+      typedef T any4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+      *reinterpret_cast<any4*>(static_cast<T*>(o.y) + at) =
+          any4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    });
     return;
   }
 #pragma unroll
@@ -98,16 +99,12 @@ DDPG_DEV void mx_bias(const MxOut& o, int j, float* b) {
 // kernels: 92 us so, 75 as a loop).
 template <int DT, int TI>
 DDPG_DEV void mx_store_tile(const MxOut& o, lds_char* strip, int i0, int j0,
-                            const f32x4 (&acc)[TI][4]) {
+                            const f32x4 (&acc)[TI][4], const float (&b)[8]) {
   typedef typename Elem<DT>::type T;
   constexpr int V = Elem<DT>::V;
   typedef __attribute__((address_space(3))) f32x4 lds_v4f;
   const int lane = threadIdx.x & 63, q = lane & 7, col = j0 + 8 * q;
   auto at = [&](int r, int unit) { return (lds_v4f*)(strip + r * 256 + ((unit ^ r) & 15) * 16); };
-  float b[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k)
-    b[k] = o.bias && col + k < o.J ? load_elem(o.bias, o.bias_dtype, col + k) : 0.f;
   static_for<TI / 4>([&](auto h_c) {
     constexpr int h = decltype(h_c)::value;
     static_for<16>([&](auto f_c) {
@@ -126,20 +123,11 @@ DDPG_DEV void mx_store_tile(const MxOut& o, lds_char* strip, int i0, int j0,
         v[k] = __fadd_rn(lo[k], b[k]);
         v[4 + k] = __fadd_rn(hi[k], b[4 + k]);
       }
-      if (o.act == DDPG_ACT_ELU) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = elu_f(v[k]);
-      } else if (o.act == DDPG_ACT_TANH) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = tanhf(v[k]);
-      }
+      mx_act(v, o.act);
       T* p = static_cast<T*>(o.y) + row * o.ldo + col;
-      if (o.vec && col + 8 <= o.J) {
+      if (col + 8 <= o.J) {  // whatever the row's alignment
 #pragma unroll
-        for (int k = 0; k < 8; k += V) {
-          const U16B u = Elem<DT>::pack(v + k);
-          *reinterpret_cast<u32x4*>(p + k) = u32x4{u.v[0], u.v[1], u.v[2], u.v[3]};
-        }
+        for (int k = 0; k < 8; k += V) *reinterpret_cast<U16B*>(p + k) = Elem<DT>::pack(v + k);
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -361,6 +349,15 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
   constexpr int NM = TI * TJ;
   static_assert(NM >= TJ + 1 + G && NM >= 2 * TJ, "gaps for the loads and the reads");
 
+  // the biases of the columns this lane will store, early (a gradient has none)
+  float bias[8];
+  {
+    const int col = (tj * C::GJ + wj * TJ) * 16 + 8 * (lane & 7);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      bias[k] = FP4 && g.o.bias && col + k < g.o.J ? load_elem(g.o.bias, g.o.bias_dtype, col + k)
+                                                   : 0.f;
+  }
   f32x4 acc[TI][TJ];
   static_for<TI * TJ>([&](auto q) {
     acc[decltype(q)::value / TJ][decltype(q)::value % TJ] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -470,7 +467,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
   __syncthreads();  // the ring is done with: it carries the results out
   by_dtype(g.o.dtype, [&](auto dt) {
     mx_store_tile<decltype(dt)::value, TI>(g.o, base + wave * 16384, (ti * C::GI + wi * TI) * 16,
-                                           (tj * C::GJ + wj * TJ) * 16, acc);
+                                           (tj * C::GJ + wj * TJ) * 16, acc, bias);
   });
 }
 
@@ -497,8 +494,13 @@ __global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemms p) {
   for (int i = 0; i < TI; ++i)
 #pragma unroll
     for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // the fragments' scales are adjacent bytes of one dword (TI, TJ: 1, 2 or 4)
+  // the fragments' scales are adjacent bytes of one dword (TI, TJ: 2 or 4)
   const int gi = pt.ti * TI, gj = pt.tj * TJ;
+  // the fragments a wave stores have one column group: its biases, loaded early
+  static_assert(NW % TJ == 0, "a wave's fragments share their columns");
+  const int jj = (gj + wave % TJ) * 16 + (lane >> 4) * 4;
+  float b[4];
+  mx_bias(g.o, jj, b);
   const uint8_t *pi[TI], *pj[TJ];
 #pragma unroll
   for (int i = 0; i < TI; ++i)
@@ -549,25 +551,31 @@ __global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemms p) {
   __syncthreads();
   // fragments wave, wave + NW ..: at most NF a wave
   constexpr int NF = (TI * TJ + NW - 1) / NW;
-  f32x4 sum[NF];
-  const bool on = wave < TI * TJ;
-#pragma unroll
-  for (int q = 0; q < NF; ++q) {
-    const int f = min(wave + q * NW, TI * TJ - 1);
-    sum[q] = part[0][f][lane];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) sum[q] += part[w][f][lane];
-  }
   constexpr int ON = TI * TJ < NW ? TI * TJ : NW;  // waves with a fragment
-  if (!FP4 && g.splits > 1 && !mx_join<NF>(g, pt, sum, threadIdx.x, ON * 64, on)) return;
-  if (!on) return;
+  const bool on = wave < TI * TJ;
+  int parts = NW;
+  if (!FP4 && g.splits > 1) {  // this block's sums joined with the other splits'
+    f32x4 sum[NF];
 #pragma unroll
-  for (int q = 0; q < NF; ++q) {
-    const int f = wave + q * NW, i = f / TJ, j = f % TJ;
-    const int jj = (gj + j) * 16 + (lane >> 4) * 4;
-    float b[4];
-    mx_bias(g.o, jj, b);
-    mx_store(g.o, (gi + i) * 16 + (lane & 15), jj, sum[q], b);
+    for (int q = 0; q < NF; ++q) {
+      const int f = min(wave + q * NW, TI * TJ - 1);
+      sum[q] = part[0][f][lane];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) sum[q] += part[w][f][lane];
+    }
+    if (!mx_join<NF>(g, pt, sum, threadIdx.x, ON * 64, on)) return;
+    if (on)
+#pragma unroll
+      for (int q = 0; q < NF; ++q) part[0][wave + q * NW][lane] = sum[q];
+    parts = 1;
+  }
+  // a loop: unrolled, the activations' code would not stay in the cache
+#pragma unroll 1
+  for (int f = wave; f < TI * TJ; f += NW) {
+    const int i = f / TJ;
+    f32x4 sum = part[0][f][lane];
+    for (int w = 1; w < parts; ++w) sum += part[w][f][lane];
+    mx_store(g.o, (gi + i) * 16 + (lane & 15), jj, sum, b);
   }
 }
 
@@ -615,6 +623,9 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(RawX x, FragOp w, int 
     xp[i] = static_cast<const T*>(x.p) + min(i * 16 + (lane & 15), x.rows - 1) * x.sr;
   const uint8_t* pj = w.p + (size_t)gj * kt * 1024 + lane * 16;
   const uint8_t* qj = w.scales + (size_t)(gj >> 2) * kt * 256 + lane * 4 + (gj & 3);
+  const int jj = gj * 16 + (lane >> 4) * 4;
+  float b[4];
+  mx_bias(o, jj, b);
   f32x4 acc[TI];
 #pragma unroll
   for (int i = 0; i < TI; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -651,9 +662,6 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(RawX x, FragOp w, int 
   f32x4 sum = part[0][wave][lane];
 #pragma unroll
   for (int s = 1; s < NW; ++s) sum += part[s][wave][lane];
-  const int jj = gj * 16 + (lane >> 4) * 4;
-  float b[4];
-  mx_bias(o, jj, b);
   mx_store(o, wave * 16 + (lane & 15), jj, sum, b);
 }
 
