@@ -10,6 +10,7 @@ Reference-interface modules:
   parameters     Parameters                            (reference parameters.py)
   ddpg           --job_name / --task_index CLI         (reference ddpg.py)
   learner        fused learner step + RCCL data parallelism
+  ops            gradient norm and clip, MXFP4 products on torch tensors
 """
 import os
 

@@ -610,7 +610,8 @@ DDPG_DEV void mx_load_block(const typename Elem<DT>::type* p, long long sc, bool
 }
 
 // y = act(x w^T + b) for at most 16 TI rows: a block makes 16 columns, its waves
-// taking every NW-th depth step, the sums joined in wave order.
+// taking every NW-th depth step, the sums joined in wave order.  Bound: latency
+// (one row, 1024 x 1024: 4.0 us with the launch; 7.9 as two launches).
 template <int DT, int TI, int NW>
 __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(RawX x, FragOp w, int kt, MxOut o) {
   __shared__ f32x4 part[NW][TI][64];
