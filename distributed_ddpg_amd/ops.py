@@ -172,6 +172,8 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, inplace=False):
     _check(lib.ddpg_clip_by_global_norm(
         l.index, _stream(l.index), l.n, l.dtype, l.ptr.buffer_info()[0], dst.buffer_info()[0],
         l.count, *l.rows, clip_norm, given, wp, nb, to))
+    if inplace:  # autograd sees the write, as it does torch's own
+        torch.autograd.graph.increment_version(out)
     it = iter(out)
     return [None if t is None else next(it) for t in t_list], norm
 

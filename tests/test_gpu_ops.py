@@ -131,6 +131,20 @@ def test_norm_strides_none_and_use_norm():
     assert abs(float(ops.global_norm([off])) / O.global_norm([off.cpu()]) - 1) < 2.0 ** -23
 
 
+def test_clip_in_place_is_seen_by_autograd():
+    a = torch.ones(8, device="cuda", requires_grad=True)
+    g = torch.full((8,), 3.0, device="cuda")
+    y = a * g  # keeps g for its backward
+    with pytest.raises(ValueError):
+        ops.clip_by_global_norm([a], 1.0)
+    ops.clip_by_global_norm([g], 1.0, inplace=True)
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+    with torch.no_grad():
+        out, _ = ops.clip_by_global_norm([a], 1e9)
+    assert torch.equal(out[0], a) and not out[0].requires_grad
+
+
 def test_clip_refuses_overlap():
     b = torch.ones(64, 64, device="cuda")
     for bad in ([b, b], [b, b[0]], [b[:, :40], b[:, 39:]], [b.view(-1)[:100], b.view(-1)[99:]],
