@@ -1525,10 +1525,11 @@ int ddpg_soft_update(ddpg_ctx* c, int mask) {
 // makes the action, both in the context's precision.
 static void mx_alloc(ddpg_ctx* c, bool train) {
   auto& m = c->mx;
+  if (m.w2 && (!train || m.ws)) return;
   auto get = [](auto*& p, size_t bytes) {
     if (p) return;
     void* q = nullptr;
-    HIP_TRY(hipMalloc(&q, std::max<size_t>(bytes, 16)));
+    HIP_TRY(hipMalloc(&q, bytes));
     HIP_TRY(hipMemset(q, 0, bytes));
     p = static_cast<std::remove_reference_t<decltype(p)>>(q);
   };
@@ -1537,7 +1538,6 @@ static void mx_alloc(ddpg_ctx* c, bool train) {
   get(m.h1, B * c->ldAH1 * 4);
   get(m.h2, B * c->ldAH2 * 4);
   get(m.snap, (c->L.actor_end - c->L.actor_begin) * 4);
-  get(m.w2, mx_bytes(c->AH2, c->AH1));
   if (train) {
     get(m.w2_train, mx_bytes(c->AH2, c->AH1));
     get(m.dh1, B * c->AH1 * 4);
@@ -1548,7 +1548,8 @@ static void mx_alloc(ddpg_ctx* c, bool train) {
       ws = std::max(ws, mx_layer_grad_ws(b, c->AH2, c->AH1));
     get(m.ws, ws);
   }
-  HIP_TRY(hipDeviceSynchronize());
+  get(m.w2, mx_bytes(c->AH2, c->AH1));
+  HIP_TRY(hipDeviceSynchronize());  // the clears are done before the ctx's stream goes on
 }
 
 // base: the actor's flat region; w2: its hidden layer, quantised
