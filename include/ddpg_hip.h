@@ -275,7 +275,8 @@ int ddpg_profile_read(ddpg_ctx* ctx, int n, char (*names)[64], double* ms, int64
  * captured into a graph and issued from any thread; outputs and workspaces are
  * the caller's and must not be shared by calls that may run at once.  Errors as
  * above, message in ddpg_global_error().  dtype: enum ddpg_dtype.
- * distributed_ddpg_amd/ops.py is the Python form.
+ * Strides (and ld below) are in elements.  distributed_ddpg_amd/ops.py is the
+ * Python form.
  *
  * A list of n tensors: dtype[i], a pointer, count[i] elements.  cols / ld
  * (both NULL, or arrays): where cols[i] > 0 tensor i is rows of cols[i]
