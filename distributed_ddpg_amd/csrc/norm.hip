@@ -180,7 +180,8 @@ static void gn_check(const GnList& l) {
       throw einval("tensor %d: %lld elements", i, (long long)l.count[i]);
     if (l.count[i] && (!l.src[i] || (l.dst && !l.dst[i]))) throw einval("tensor %d: null", i);
     if (l.cols && l.cols[i]) {
-      if (l.cols[i] < 1 || l.cols[i] > INT32_MAX || l.ld[i] < 0 || l.count[i] % l.cols[i])
+      if (l.cols[i] < 1 || l.cols[i] > INT32_MAX || l.ld[i] < 0 || l.count[i] % l.cols[i] ||
+          l.ld[i] > (1ll << 56) / std::max<int64_t>(1, l.count[i] / l.cols[i]))
         throw einval("tensor %d: rows of %lld, %lld apart, %lld elements", i,
                      (long long)l.cols[i], (long long)l.ld[i], (long long)l.count[i]);
     }
@@ -217,7 +218,7 @@ static void gn_check_disjoint(const GnList& l, const float* use_norm) {
       const int i = r[a].i, j = r[b].i;
       const int64_t ei = elem_size(l.dtype[i]), ej = elem_size(l.dtype[j]);
       bool apart = false;
-      if (l.cols && l.cols[i] && l.cols[j] && l.ld[i] * ei == l.ld[j] * ej) {
+      if (l.cols && l.cols[i] && l.cols[j] && l.ld[i] && l.ld[i] * ei == l.ld[j] * ej) {
         const uintptr_t pitch = (uintptr_t)(l.ld[i] * ei);
         const uintptr_t at = (r[b].lo - r[a].lo) % pitch;  // j's row within i's pitch
         apart = at >= (uintptr_t)(l.cols[i] * ei) && at + (uintptr_t)(l.cols[j] * ej) <= pitch;

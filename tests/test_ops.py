@@ -73,6 +73,19 @@ def test_norm_entry_refusals():
     refused(clip(1.0, 2, at, at, two, cols, ld), "overlap")
 
 
+def test_single_rows_without_a_pitch():
+    """A single row may name any distance to the next, 0 too."""
+    dt, n = arr(ctypes.c_int, 0, 0), arr(ctypes.c_int64, 8, 8)
+    at = arr(ctypes.c_void_p, 4096, 4096 + 16)
+    for pitch in (0, 4, 1 << 56):
+        ld = arr(ctypes.c_int64, pitch, pitch)
+        refused(L.ddpg_clip_by_global_norm(0, None, 2, dt, at, at, n, n, ld, 1.0, None, 1, 1 << 20,
+                                           1), "tensors 0 and 1 overlap")
+    ld = arr(ctypes.c_int64, 1 << 56, 1 << 56)  # two rows: their span leaves 64 bits
+    refused(L.ddpg_clip_by_global_norm(0, None, 2, dt, at, at, n, arr(ctypes.c_int64, 4, 4), ld, 1.0,
+                                       None, 1, 1 << 20, 1), "rows of 4")
+
+
 def test_mx_entry_refusals():
     big = (1 << 24) + 1
     a, b = ctypes.c_size_t(), ctypes.c_size_t()
