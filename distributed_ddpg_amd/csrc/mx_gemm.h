@@ -83,10 +83,33 @@ DDPG_DEV void mx_store(const MxOut& o, int i, int j, const f32x4& d, const float
     if (j + r < o.J) store_elem(o.y, o.dtype, at + r, v[r]);
 }
 
-DDPG_DEV void mx_bias(const MxOut& o, int j, float* b) {
+// The biases of N columns from j on, as their bits: loaded first and converted
+// last, so that nothing waits for them before the operands are on their way
+// (columns past the last repeat its bias, and are not stored).
+template <int N>
+DDPG_DEV void mx_bias(const MxOut& o, int j, unsigned (&u)[N]) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-    b[r] = o.bias && j + r < o.J ? load_elem(o.bias, o.bias_dtype, j + r) : 0.f;
+  for (int k = 0; k < N; ++k) u[k] = 0;
+  if (!o.bias) return;
+  if (o.bias_dtype == T_FP32) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) u[k] = static_cast<const unsigned*>(o.bias)[min(j + k, o.J - 1)];
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      u[k] = static_cast<const unsigned short*>(o.bias)[min(j + k, o.J - 1)];
+  }
+}
+template <int N>
+DDPG_DEV void mx_bias_values(const MxOut& o, const unsigned (&u)[N], float (&b)[N]) {
+  by_dtype(o.bias_dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      b[k] = DT == T_FP32   ? __uint_as_float(u[k])
+             : DT == T_BF16 ? __uint_as_float(u[k] << 16)
+                            : (float)__builtin_bit_cast(_Float16, (unsigned short)u[k]);
+  });
 }
 
 // A wave's TI x 4 fragments to the output by whole rows: 64 rows at a time go
@@ -169,28 +192,34 @@ DDPG_DEV void mx_db(const MxGemms& p, int b, double (&red)[NW][64]) {
 // eight rows of tiles down before it steps across, so that the tiles an XCD
 // works on at once share their operands in its L2.
 DDPG_DEV void tile_of(int lin, int ni, int nj, int& ti, int& tj) {
-  const int n = ni * nj;
-  const int x = lin & 7, q = n >> 3, r = n & 7;
-  const int t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (lin >> 3);
-  const int band = t / (8 * nj), in = t - band * 8 * nj;
-  const int rows = min(8, ni - band * 8);
-  ti = band * 8 + in % rows;
-  tj = in / rows;
+  const unsigned n = ni * nj;
+  const unsigned x = lin & 7, q = n >> 3, r = n & 7;
+  const unsigned t = x * q + min(x, r) + ((unsigned)lin >> 3);
+  const unsigned band = t / (8u * nj), in = t - band * 8 * nj;
+  const unsigned rows = min(8u, ni - band * 8), d = in / rows;
+  ti = band * 8 + in - d * rows;
+  tj = d;
 }
 
 // Which of a product's blocks this is: tile, split and its depth steps.
 struct MxPart {
   int ti, tj, tile, split, k0, n;
 };
-DDPG_DEV MxPart mx_part(const MxGemm& g, int lin, int bi, int bj) {
-  const int ni = (g.o.I + bi - 1) / bi, nj = (g.o.J + bj - 1) / bj, nt = ni * nj;
+template <bool FP4, int BI, int BJ>
+DDPG_DEV MxPart mx_part(const MxGemm& g, unsigned lin) {
+  const unsigned ni = (unsigned)(g.o.I + BI - 1) / BI, nj = (unsigned)(g.o.J + BJ - 1) / BJ;
   MxPart p;
-  p.split = lin / nt;
-  tile_of(lin - p.split * nt, ni, nj, p.ti, p.tj);
+  p.split = p.k0 = 0;
+  p.n = g.kt * g.planes;
+  if (!FP4 && g.splits > 1) {  // at most 32, of at most 3 * 2^19 steps
+    const unsigned nk = p.n;
+    p.split = lin / (ni * nj);
+    lin -= p.split * ni * nj;
+    p.k0 = nk * p.split / g.splits;
+    p.n = nk * (p.split + 1) / g.splits - p.k0;
+  }
+  tile_of(lin, ni, nj, p.ti, p.tj);
   p.tile = p.ti * nj + p.tj;
-  const long long nk = (long long)g.kt * g.planes;
-  p.k0 = (int)(nk * p.split / g.splits);
-  p.n = (int)(nk * (p.split + 1) / g.splits) - p.k0;
   return p;
 }
 
@@ -273,6 +302,7 @@ struct RingCfg {
   static constexpr int SLOT = (GI + GJ) * 1024 + SP * 256;
   static constexpr int LDS = NS * SLOT;
   static_assert(PW * NW == GI + GJ && SW * NW == SP && TI % 4 == 0 && TJ % 4 == 0, "whole pieces");
+  static_assert(GI % PW == 0 && (!FP4 || PW == 4 * SW), "a wave's pieces are of one operand");
   static_assert(TJ == 4 && LDS >= NW * 16384, "mx_store_tile");
   static_assert(LDS <= 160 * 1024, "LDS");
   static_assert((GI + GJ) * 1024 + SP * 256 < 65536, "LDS offsets are immediates");
@@ -300,34 +330,31 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ, wj = wave % WJ;
-  const MxPart pt = mx_part(g, blockIdx.x - (second ? p.end[0] : 0), C::GI * 16, C::GJ * 16);
+  const MxPart pt =
+      mx_part<FP4, C::GI * 16, C::GJ * 16>(g, blockIdx.x - (second ? p.end[0] : 0));
   const int ti = pt.ti, tj = pt.tj, nk = pt.n;
-  int jk = pt.k0 % max(g.kt, 1);  // J's depth step of the next load (I's planes go on, J's repeat)
+  // J's depth step of the next load (I's planes go on, J's repeat)
+  int jk = FP4 ? 0 : (unsigned)pt.k0 % max((unsigned)g.kt, 1u);
 
   // this wave's pieces of a step: source of the next step to load, LDS place.
   // The sources are the same for all lanes (scalar registers, scalar adds), a
   // lane's place in a piece is its own.
   // Row groups past the operand's last are read from the last one's place
   // (their results are not stored).
+  const bool isj = wave >= C::GI / C::PW;  // a wave's pieces are of one operand
+  const FragOp& op = isj ? g.J : g.I;
   const uint8_t* src[C::PW];
   const uint8_t* ssrc[C::SW + 1];
-  bool isj[C::PW];
+  {
+    const int g0 = isj ? tj * C::GJ - C::GI + wave * C::PW : ti * C::GI + wave * C::PW;
+    const size_t pitch = (size_t)g.kt * (isj ? 1 : g.planes) * 1024;
+    const uint8_t* at = op.p + (size_t)(isj ? jk : pt.k0) * 1024;
 #pragma unroll
-  for (int p = 0; p < C::PW; ++p) {
-    const int f = wave * C::PW + p;
-    isj[p] = f >= C::GI;
-    const int grp = isj[p] ? min(tj * C::GJ + f - C::GI, g.J.groups - 1)
-                           : min(ti * C::GI + f, g.I.groups - 1);
-    src[p] = (isj[p] ? g.J.p + ((size_t)grp * g.kt + jk) * 1024
-                     : g.I.p + ((size_t)grp * g.kt * g.planes + pt.k0) * 1024);
-  }
+    for (int p = 0; p < C::PW; ++p) src[p] = at + min(g0 + p, op.groups - 1) * pitch;
+    const int s0 = isj ? (tj * C::GJ - C::GI) / 4 + wave * C::SW : ti * (C::GI / 4) + wave * C::SW;
 #pragma unroll
-  for (int p = 0; p < C::SW; ++p) {
-    const int f = wave * C::SW + p;
-    const bool j = f >= C::GI / 4;
-    const int grp = j ? min(tj * (C::GJ / 4) + f - C::GI / 4, g.J.groups / 4 - 1)
-                      : min(ti * (C::GI / 4) + f, g.I.groups / 4 - 1);
-    ssrc[p] = (j ? g.J.scales : g.I.scales) + ((size_t)grp * g.kt + pt.k0) * 256;
+    for (int p = 0; p < C::SW; ++p)
+      ssrc[p] = op.scales + (size_t)min(s0 + p, op.groups / 4 - 1) * g.kt * 256;
   }
   lds_char* const base = (lds_char*)smem;
   const unsigned l16 = lane * 16, l4 = lane * 4;
@@ -336,7 +363,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
     if constexpr (p < C::PW) {
       lds_load16(src[p] + l16, base + slot * C::SLOT + (wave * C::PW + p) * 1024);
       src[p] += 1024;
-      if (!FP4 && isj[p] && jk + 1 == g.kt) src[p] -= (size_t)g.kt * 1024;
+      if (!FP4 && isj && jk + 1 == g.kt) src[p] -= (size_t)g.kt * 1024;
     } else {
       constexpr int q = p - C::PW;
       lds_load4(ssrc[q] + l4,
@@ -349,15 +376,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
   constexpr int NM = TI * TJ;
   static_assert(NM >= TJ + 1 + G && NM >= 2 * TJ, "gaps for the loads and the reads");
 
-  // the biases of the columns this lane will store, early (a gradient has none)
-  float bias[8];
-  {
-    const int col = (tj * C::GJ + wj * TJ) * 16 + 8 * (lane & 7);
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      bias[k] = FP4 && g.o.bias && col + k < g.o.J ? load_elem(g.o.bias, g.o.bias_dtype, col + k)
-                                                   : 0.f;
-  }
+  unsigned bias[8] = {};  // of the columns this lane will store (a gradient has none)
+  if (FP4) mx_bias(g.o, (tj * C::GJ + wj * TJ) * 16 + 8 * (lane & 7), bias);
   f32x4 acc[TI][TJ];
   static_for<TI * TJ>([&](auto q) {
     acc[decltype(q)::value / TJ][decltype(q)::value % TJ] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -410,7 +430,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
       constexpr int SET = decltype(set_c)::value;
       constexpr bool RT = decltype(rt_c)::value;
       using Other = std::integral_constant<int, SET ^ 1>;
-      const bool next = !RT || s + 1 < nk, stage = !RT || s + NS < nk;
+      const bool next = true, stage = !RT || s + NS < nk;
       if (RT && s + NS > nk)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       else
@@ -464,10 +484,12 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
   }
   if (!FP4 && g.splits > 1 && !mx_join<TI * TJ>(g, pt, &acc[0][0], threadIdx.x, C::NT, true))
     return;
+  float b[8];
+  mx_bias_values(g.o, bias, b);
   __syncthreads();  // the ring is done with: it carries the results out
   by_dtype(g.o.dtype, [&](auto dt) {
     mx_store_tile<decltype(dt)::value, TI>(g.o, base + wave * 16384, (ti * C::GI + wi * TI) * 16,
-                                           (tj * C::GJ + wj * TJ) * 16, acc, bias);
+                                           (tj * C::GJ + wj * TJ) * 16, acc, b);
   });
 }
 
@@ -487,7 +509,7 @@ __global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemms p) {
   const MxGemm& g = p.g[second];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const MxPart pt = mx_part(g, blockIdx.x - (second ? p.end[0] : 0), TI * 16, TJ * 16);
+  const MxPart pt = mx_part<FP4, TI * 16, TJ * 16>(g, blockIdx.x - (second ? p.end[0] : 0));
   const int nk = pt.n;
   f32x4 acc[TI][TJ];
 #pragma unroll
@@ -499,8 +521,8 @@ __global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemms p) {
   // the fragments a wave stores have one column group: its biases, loaded early
   static_assert(NW % TJ == 0, "a wave's fragments share their columns");
   const int jj = (gj + wave % TJ) * 16 + (lane >> 4) * 4;
-  float b[4];
-  mx_bias(g.o, jj, b);
+  unsigned bias[4] = {};
+  if (FP4) mx_bias(g.o, jj, bias);
   const uint8_t *pi[TI], *pj[TJ];
 #pragma unroll
   for (int i = 0; i < TI; ++i)
@@ -569,6 +591,8 @@ __global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemms p) {
       for (int q = 0; q < NF; ++q) part[0][wave + q * NW][lane] = sum[q];
     parts = 1;
   }
+  float b[4];
+  mx_bias_values(g.o, bias, b);
   // a loop: unrolled, the activations' code would not stay in the cache
 #pragma unroll 1
   for (int f = wave; f < TI * TJ; f += NW) {
@@ -625,8 +649,8 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(RawX x, FragOp w, int 
   const uint8_t* pj = w.p + (size_t)gj * kt * 1024 + lane * 16;
   const uint8_t* qj = w.scales + (size_t)(gj >> 2) * kt * 256 + lane * 4 + (gj & 3);
   const int jj = gj * 16 + (lane >> 4) * 4;
-  float b[4];
-  mx_bias(o, jj, b);
+  unsigned bias[4];
+  mx_bias(o, jj, bias);
   f32x4 acc[TI];
 #pragma unroll
   for (int i = 0; i < TI; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -663,6 +687,8 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(RawX x, FragOp w, int 
   f32x4 sum = part[0][wave][lane];
 #pragma unroll
   for (int s = 1; s < NW; ++s) sum += part[s][wave][lane];
+  float b[4];
+  mx_bias_values(o, bias, b);
   mx_store(o, wave * 16 + (lane & 15), jj, sum, b);
 }
 
