@@ -41,7 +41,8 @@ struct MxGemm {
 };
 
 // One launch: n products (blocks 0 .. end[0] - 1, .. end[1] - 1), then 64 columns
-// a block of a bias gradient's last sum.
+// a block of a bias gradient's last sum.  A launch of fp4 is g[0] alone, so that its
+// blocks take all arguments at fixed places, with one wait.
 struct MxGemms {
   MxGemm g[2];
   int n, end[2];
@@ -321,11 +322,11 @@ template <bool FP4, int WI, int WJ, int TI, int TJ, int NS>
 __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
   using C = RingCfg<FP4, WI, WJ, TI, TJ, NS>;
   __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
-  if ((int)blockIdx.x >= p.end[1]) {
+  if (!FP4 && (int)blockIdx.x >= p.end[1]) {
     mx_db<C::NW>(p, blockIdx.x - p.end[1], *reinterpret_cast<double(*)[C::NW][64]>(smem));
     return;
   }
-  const bool second = (int)blockIdx.x >= p.end[0];
+  const bool second = !FP4 && (int)blockIdx.x >= p.end[0];
   const MxGemm& g = p.g[second];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -501,11 +502,11 @@ template <bool FP4, int TI, int TJ, int NW, int PF>
 __global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemms p) {
   __shared__ f32x4 part[NW][TI * TJ][64];
   static_assert(TI * TJ < NW || TI * TJ % NW == 0, "whole fragments a wave");
-  if ((int)blockIdx.x >= p.end[1]) {
+  if (!FP4 && (int)blockIdx.x >= p.end[1]) {
     mx_db<NW>(p, blockIdx.x - p.end[1], *reinterpret_cast<double(*)[NW][64]>(part));
     return;
   }
-  const bool second = (int)blockIdx.x >= p.end[0];
+  const bool second = !FP4 && (int)blockIdx.x >= p.end[0];
   const MxGemm& g = p.g[second];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
