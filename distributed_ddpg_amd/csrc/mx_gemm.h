@@ -51,6 +51,24 @@ struct MxGemms {
   int db_parts, db_n;
 };
 
+// g[0] or g[1], field by field: loaded at once from fixed places, then selected (a
+// load from a selected address waits a second time for the arguments' memory).
+template <bool FP4>
+DDPG_DEV MxGemm mx_pick(const MxGemms& p, bool second) {
+  if constexpr (FP4) return p.g[0];
+  const MxGemm &a = p.g[0], &b = p.g[1];
+  auto pick = [&](auto x, auto y) { return second ? y : x; };
+  return {{pick(a.I.p, b.I.p), nullptr, pick(a.I.groups, b.I.groups)},
+          {pick(a.J.p, b.J.p), nullptr, pick(a.J.groups, b.J.groups)},
+          pick(a.kt, b.kt),
+          a.planes,
+          {pick(a.o.y, b.o.y), nullptr, a.o.ldo, pick(a.o.I, b.o.I), a.o.J,
+           pick(a.o.dtype, b.o.dtype), 0, DDPG_ACT_NONE},
+          pick(a.splits, b.splits),
+          pick(a.slab, b.slab),
+          pick(a.tickets, b.tickets)};
+}
+
 template <int N>
 DDPG_DEV void mx_act(float (&v)[N], int act) {
   if (act == DDPG_ACT_ELU) {
@@ -327,7 +345,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void mx_tile_kernel(MxGemms p) {
     return;
   }
   const bool second = !FP4 && (int)blockIdx.x >= p.end[0];
-  const MxGemm& g = p.g[second];
+  const MxGemm g = mx_pick<FP4>(p, second);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ, wj = wave % WJ;
@@ -507,7 +525,7 @@ __global__ __launch_bounds__(64 * NW) void mx_split_kernel(MxGemms p) {
     return;
   }
   const bool second = !FP4 && (int)blockIdx.x >= p.end[0];
-  const MxGemm& g = p.g[second];
+  const MxGemm g = mx_pick<FP4>(p, second);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const MxPart pt = mx_part<FP4, TI * 16, TJ * 16>(g, blockIdx.x - (second ? p.end[0] : 0));
