@@ -229,7 +229,7 @@ DDPG_DEV void mx_dy(const MxPrep& a, int b, float (&t)[64][65], float (&red)[4][
     a.part[(size_t)mb * N + n0 + l] = ((red[0][l] + red[1][l]) + red[2][l]) + red[3][l];
   // 4 row groups x 2 depth steps: a wave takes row group w
   auto put = [&](uint8_t* out, int grp, int steps, int s0, auto at) {
-#pragma unroll
+#pragma unroll 1
     for (int d = 0; d < 2; ++d) {
       bf16x8 f[P];
 #pragma unroll
