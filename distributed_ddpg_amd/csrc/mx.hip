@@ -305,10 +305,10 @@ void mx_quantize_launch(hipStream_t st, int dtype, const void* x, int rows, int 
   HIP_TRY(hipGetLastError());
 }
 
-// How each of the kernels does: fp4 16384 x 8192 x 8192 490 us (4.5 PFLOP/s) on 256 x
-// 256 tiles, bf16 8192 x 8192 x 8192 741 us (1.48 PFLOP/s, both at the power limit, the
-// clock below 2 GHz); fp4 2048 x 2048 x 2048 11.5 us (1.5 PFLOP/s) on 128 x 128, 512 x
-// 4096 x 4096 13.1 us on 64 x 64, 256 x 1024 x 1024 4.4 us on 32 x 32.
+// How each of the kernels does: fp4 16384 x 8192 x 8192 487 us (4.5 PFLOP/s) on 256 x
+// 256 tiles, bf16 8192 x 4096 x 4096 twice in 385 us (1.43 PFLOP/s, both at the power
+// limit, the clock below 2 GHz); fp4 2048 x 2048 x 2048 10.8 us (1.6 PFLOP/s) on 128 x
+// 128, 512 x 4096 x 4096 12.3 us on 64 x 64, 256 x 1024 x 1024 4.1 us on 32 x 32.
 //
 // The kernels of a product: tiles of 256 x 256 and 128 x 128 through LDS, and 64 x 64
 // and 32 x 32 with the depth split over a block's 4 and 8 waves.
@@ -353,19 +353,20 @@ void mx_linear_launch(hipStream_t st, const MxMat& x, const MxMat& w, const MxOu
   MxGemms p{};
   p.n = 1;
   p.g[0] = {mx_op(x), mx_op(w), x.kt(), 1, o, 1, nullptr, nullptr};
-  // Measured on 60 shapes, us: 256 x 4096 x 1024 5.0 on 32 x 32 tiles, 9.5 on 64; 512 x
-  // 4096 x 4096 13.1 on 64 x 64, 20.2 on 32, 19.5 on 128; 4096 x 1024 x 1024 11.3 on 128 x
-  // 128, 14.7 on 64, 17.1 on 256; 8192 x 2048 x 2048 26.5 on 256 x 256, 32.8 on 128
+  // Measured on 60 shapes, us: 640 x 1024 x 1024 5.7 on 32 x 32 tiles, 6.0 on 64; 512 x
+  // 4096 x 4096 12.3 on 64 x 64, 18.8 on 32, 13.3 on 128; 4096 x 1024 x 1024 8.8 on 128 x
+  // 128, 12.0 on 64, 14.8 on 256; 8192 x 2048 x 2048 24.0 on 256 x 256, 26.7 on 128
   auto tiles = [&](int pick) { return mx_tiles(o.I, o.J, kMxTile[pick]); };
   mx_gemm_launch<true>(st, p, tiles(MX_256) >= 256  ? MX_256
-                              : tiles(MX_32) <= 384 ? MX_32
+                              : tiles(MX_32) <= 640 ? MX_32
                               : tiles(MX_64) <= 512 ? MX_64
                                                     : MX_128);
 }
 
 // Whether the rows of x are quantised by every block of 16 columns of the
-// product.  A row of 8192 values: 7.5 us so, 9.5 in two launches; 16 rows of 2048 6.5
-// and 7.1, of 4096 10.2 and 7.8; 64 of 512 7.6 and 6.8 (and the launch's host time).
+// product.  A row of 8192 values: 7.6 us so, 8.8 in two launches; 16 rows of 512 4.7
+// and 5.7, of 2048 6.5 and 6.3, of 4096 10.2 and 7.2; 64 of 512 7.4 and 5.8 (a second
+// launch costs the host 2.5 us besides).
 static bool mx_rows_ok(int64_t M, int64_t K) { return M <= 64 && M * K <= 32768; }
 void mx_linear_rows_launch(hipStream_t st, int dtype, const void* x, long long sr, long long sc,
                            int M, int K, const MxMat& w, const MxOut& o) {
@@ -400,14 +401,14 @@ static MxGradPlan mx_grad_plan(int dtype, int M, int N, int K, bool dx, bool dw,
   auto tiles = [&](int q, int pick) { return mx_tiles(I[q], K, kMxTile[pick]); };
   auto all = [&](int pick) { return tiles(0, pick) * steps[0] + tiles(1, pick) * steps[1]; };
   // Each kernel up to the work (a tile costs about 16 depth steps besides its own)
-  // it is best at; us, bf16: 1362 x 195 x 2659 26.3 on 64 x 64 tiles, 26.5 on 32, 37.9 on 128;
-  // 2048 x 2048 x 2048 57.8 on 128 x 128, 71.1 on 64, 72.6 on 256; 4096 x 2048 x 2048 95.4 on 256
-  // x 256, 106.7 on 128
+  // it is best at; us, bf16: 1362 x 195 x 2659 24.2 on 64 x 64 tiles, 24.9 on 32, 28.2 on 128;
+  // 2048 x 2048 x 2048 46.2 on 128 x 128, 62.8 on 64, 61.2 on 256; 8192 x 2048 x 2048 136 on
+  // 256 x 256, 141 on 128 (4096 x 2048 x 2048 89 and 80)
   auto cost = [&](int pick) { return all(pick) + 16 * (tiles(0, pick) + tiles(1, pick)); };
-  w.pick = cost(MX_256) >= 16000    ? MX_256
-           : cost(MX_32) <= 40000   ? MX_32
-           : cost(MX_64) <= 160000  ? MX_64
-                                    : MX_128;
+  w.pick = cost(MX_256) >= 32000  ? MX_256
+           : cost(MX_32) <= 40000 ? MX_32
+           : cost(MX_64) <= 40000 ? MX_64
+                                  : MX_128;
   // a block's depth: an equal share of a launch that fills the chip, but no less
   // than what makes the join worth it
   const long long least[] = {32, 24, 32, 64}, fill[] = {256, 256, 512, 512};

@@ -425,11 +425,13 @@ def test_linear_tiles(M, K, N, dt, act):
     assert (err <= linear_tol(want, s, K, DT[dt], 1.0 if act else 0.0)).all(), float(err.max())
 
 
-@pytest.mark.parametrize("M,K,N,dt", [(1100, 900, 1050, "fp16"),   # 64 x 64 tiles
-                                      (2050, 2049, 2047, "bf16"),  # 128 x 128
+@pytest.mark.parametrize("M,K,N,dt", [(700, 650, 900, "fp16"),     # 64 x 64 tiles
+                                      (1100, 900, 1050, "fp16"),   # 128 x 128
+                                      (2050, 2049, 2047, "bf16"),
                                       (8192, 4096, 64, "bf16"),    # and dW in 11 splits
-                                      (8190, 65, 4095, "fp32"),    # 256 x 256, 4 and 8 splits
-                                      (4099, 2051, 2040, "fp32"),
+                                      (8190, 65, 4095, "fp32"),
+                                      (4099, 2051, 2040, "fp32"),  # 256 x 256, dW in 2 splits
+                                      (16001, 300, 4096, "fp32"),  # in 4
                                       (8000, 17, 5, "fp32")])      # 32 x 32, dW in 12 splits
 def test_linear_grad_tiles(M, K, N, dt):
     x, w, dy = rnd(M, K, seed=1), rnd(N, K, seed=2), rnd(M, N, dt=dt, seed=3)
