@@ -282,6 +282,33 @@ def test_linear_large_and_tiny_scales():
 
 
 # ---------------------------------------------------------------- gradient
+@pytest.mark.parametrize("M", [1, 100, 2048])  # each kernel's epilogue
+def test_activations_over_their_range(M):
+    """act(0 + bias): the activation alone.  elu: exp(x) - 1, its argument's rounding
+    moves it by |x| e^x 2^-24 <= 2^-25, exp by 2^-23, the difference by 2^-25.  tanh by
+    1 - 2 r: e's error enters as 2 (r - r^2) (2^-23 + 2 |x| 2^-24) <= 2^-23, the sum's and
+    r's as 2 r (2^-24 + 2^-23) <= 0.81 2^-23 (r < 0.27), the last rounding as 2^-25; its
+    polynomial, below 0.5, is within 2^-23 of the value (and half a step)."""
+    b = torch.cat([torch.linspace(-12, 12, 1999), torch.linspace(-0.6, 0.6, 2001),
+                   torch.logspace(-38, 2, 47), -torch.logspace(-38, 2, 47),
+                   torch.tensor([0.0, -0.0, 0.5, -0.5, 88.0, -104.0, 1e30, -1e30, math.inf,
+                                 -math.inf, math.nan])]).float()
+    x, wq = torch.zeros(M, 1, device="cuda"), ops.mx_quantize(torch.zeros(len(b), 1, device="cuda"))
+    t = b.double()
+    for act, want, tol in (("elu", torch.where(t < 0, torch.expm1(t), t),
+                            torch.where(t < 0, 2.0 ** -22, 0.0)),
+                           ("tanh", torch.tanh(t), torch.where(t.abs() < 0.5,
+                                                               t.abs() * 1.5 * 2.0 ** -23,
+                                                               2.25 * 2.0 ** -23))):
+        y = ops.mx_linear(x, wq, b.cuda(), act).cpu().double()
+        assert torch.equal(y[0], y[-1]) or torch.equal(y[0].isnan(), y[-1].isnan())
+        for r in (y[0], y[-1]):
+            assert torch.equal(r.isnan(), t.isnan())
+            err = (r - want).abs()[:-1]
+            err = torch.where(want[:-1] == r[:-1], 0.0, err)  # the infinite ones
+            assert (err <= tol[:-1] + 2.0 ** -126).all(), (act, float((err - tol[:-1]).max()))
+
+
 @pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("M,K,N", [(1, 1, 1), (1, 300, 200), (3, 64, 64), (64, 32, 128),
                                    (65, 129, 63), (100, 400, 300), (1001, 400, 300),
