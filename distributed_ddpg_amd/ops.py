@@ -25,7 +25,6 @@ from . import _lib
 from ._lib import lib
 
 _DTYPES = {torch.float32: _lib.FP32, torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
-_STRIDED = {torch.strided}
 _ACTS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "elu": _lib.ACT_ELU, "tanh": _lib.ACT_TANH}
 
 
@@ -89,13 +88,16 @@ class _List:
         if not src:
             raise ValueError("t_list: no tensor in the list")
         # whole-list checks (a list has hundreds of tensors); what fails one is
-        # named by the tensor's own check
+        # named by the tensor's own check (a sparse one has no data_ptr)
         try:
-            dt = array("i", [_DTYPES[t.dtype] for t in src])
+            dt = {t.dtype for t in src}
+            dt = (array("i", [_DTYPES[dt.pop()]]) * len(src) if len(dt) == 1
+                  else array("i", [_DTYPES[t.dtype] for t in src]))
             index = {t.get_device() for t in src}
-            fine = (len(index) == 1 and min(index) >= 0 and {t.layout for t in src} == _STRIDED
+            self.ptr = array("Q", [t.data_ptr() for t in src])
+            fine = (len(index) == 1 and min(index) >= 0
                     and not (torch.is_grad_enabled() and any([t.requires_grad for t in src])))
-        except (AttributeError, KeyError, TypeError):
+        except (AttributeError, KeyError, TypeError, RuntimeError):
             fine = False
         if not fine:
             for i, t in enumerate(src):
@@ -115,10 +117,10 @@ class _List:
                                      "rows" % (i, tuple(t.stride())))
                 if rc is None:
                     src[i] = t.contiguous()
+                    self.ptr[i] = src[i].data_ptr()
                 else:
                     cols[i], ld[i] = rc
         self.cols = cols
-        self.ptr = array("Q", [t.data_ptr() for t in src])
         self._held = (dt, cols, ld, array("q", [t.numel() for t in src]))
         self.n = len(src)
         addr = lambda a: None if a is None else a.buffer_info()[0]

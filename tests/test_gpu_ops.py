@@ -145,6 +145,18 @@ def test_clip_in_place_is_seen_by_autograd():
     assert torch.equal(out[0], a) and not out[0].requires_grad
 
 
+def test_lists_refuse_what_has_no_dense_storage():
+    a = torch.ones(4, 4, device="cuda")
+    for bad in (a.to_sparse(), a.to_sparse_csr(), a.to("meta"), a.int(), a.cpu()):
+        for ts in ([bad], [a, bad], [bad, a]):
+            with pytest.raises(ValueError):
+                ops.global_norm(ts)
+            with pytest.raises(ValueError):
+                ops.clip_by_global_norm(ts, 1.0)
+    mixed = [2 * a, a.half(), a.bfloat16(), a.t()[1:], a.half()]  # 64 + 16 + 16 + 12 + 16 = 124
+    assert abs(float(ops.global_norm(mixed)) - 124 ** 0.5) <= 12 * 2.0 ** -24
+
+
 def test_clip_refuses_overlap():
     b = torch.ones(64, 64, device="cuda")
     for bad in ([b, b], [b, b[0]], [b[:, :40], b[:, 39:]], [b.view(-1)[:100], b.view(-1)[99:]],
