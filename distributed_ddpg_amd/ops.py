@@ -46,6 +46,9 @@ def _tensor(name, t):
     code = _DTYPES.get(t.dtype)
     if code is None or t.layout is not torch.strided:
         raise ValueError("%s: %s is none of float32, bfloat16, float16" % (name, t.dtype))
+    if t.is_neg():
+        raise ValueError("%s is a negated view (of a conjugate's imaginary part); pass "
+                         ".resolve_neg()" % name)
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s requires grad and the operator has no autograd formula; call it "
                          "under torch.no_grad() or pass .detach()" % name)
@@ -95,8 +98,9 @@ class _List:
                   else array("i", [_DTYPES[t.dtype] for t in src]))
             index = {t.get_device() for t in src}
             self.ptr = array("Q", [t.data_ptr() for t in src])
-            fine = (len(index) == 1 and min(index) >= 0
-                    and not (torch.is_grad_enabled() and any([t.requires_grad for t in src])))
+            fine = len(index) == 1 and min(index) >= 0 and not (
+                any([t.requires_grad or t.is_neg() for t in src]) if torch.is_grad_enabled()
+                else any(map(torch.Tensor.is_neg, src)))
         except (AttributeError, KeyError, TypeError, RuntimeError):
             fine = False
         if not fine:

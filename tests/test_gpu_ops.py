@@ -157,6 +157,21 @@ def test_lists_refuse_what_has_no_dense_storage():
     assert abs(float(ops.global_norm(mixed)) - 124 ** 0.5) <= 12 * 2.0 ** -24
 
 
+def test_negated_views_are_refused():
+    """A float view whose memory holds the opposite sign."""
+    z = torch.complex(torch.ones(64, 64), 2 * torch.ones(64, 64)).cuda().conj()
+    wq = ops.mx_quantize(torch.ones(64, 64, device="cuda"))
+    for v in (z.imag, z.imag[:1, :1]):
+        assert v.is_neg()
+        for f in (lambda: ops.clip_by_global_norm([v], 1.0), lambda: ops.global_norm([z.real, v]),
+                  lambda: ops.mx_quantize(v), lambda: ops.mx_linear(v, wq),
+                  lambda: ops.mx_linear_grad(v, wq, wq)):
+            with pytest.raises(ValueError):
+                f()
+    same(ops.mx_quantize(z.imag.resolve_neg()).dequantize(), torch.full((64, 64), -2.0).double())
+    same(ops.mx_quantize(z.real).dequantize(), torch.ones(64, 64).double())
+
+
 def test_clip_refuses_overlap():
     b = torch.ones(64, 64, device="cuda")
     for bad in ([b, b], [b, b[0]], [b[:, :40], b[:, 39:]], [b.view(-1)[:100], b.view(-1)[99:]],
