@@ -60,7 +60,7 @@ def _clip_norm(x):
     """A clip as the C call takes it: 0 for none."""
     if x is None:
         return 0.0
-    if not x > 0:
+    if not x >= 2.0 ** -149:  # of float32 (0 would mean no clip)
         raise ValueError("gradient clip %r is not a norm > 0 (None: no clip)" % (x,))
     return float(x)
 

@@ -86,6 +86,15 @@ def test_single_rows_without_a_pitch():
                                        None, 1, 1 << 20, 1), "rows of 4")
 
 
+def test_learner_clip_values():
+    from distributed_ddpg_amd.networks import _clip_norm
+    assert [_clip_norm(x) for x in (None, 2, 2.0 ** -149, float("inf"))] == [
+        0.0, 2.0, 2.0 ** -149, float("inf")]
+    for bad in (0, -1.0, float("nan"), 1e-50):  # 1e-50 is 0, no clip, in float32
+        with pytest.raises(ValueError):
+            _clip_norm(bad)
+
+
 def test_mx_entry_refusals():
     big = (1 << 24) + 1
     a, b = ctypes.c_size_t(), ctypes.c_size_t()
