@@ -17,6 +17,7 @@ tensor that requires grad is refused while grad mode is on.  Arguments of the
 wrong shape, type or device raise ValueError, the library's own refusals
 DDPGError.
 """
+import operator
 from array import array
 
 import torch
@@ -185,28 +186,67 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, inplace=False):
 
 
 # ---------------------------------------------------------------- MXFP4
+def _mx_bytes(rows, cols):
+    return -(-rows // 64) * -(-cols // 128) * 4352
+
+
+_MX_MAX = 1 << 24  # rows, columns
+
+
 class MXTensor:
     """A [rows, cols] matrix in MXFP4: 4-bit codes and a scale byte for 32 of
     them along a row, in the order the matrix instructions read (an opaque buffer;
-    .dequantize() gives the values).  17/32 byte a value."""
+    .dequantize() gives the values).  17/32 byte a value.
 
-    __slots__ = ("buffer", "shape", "_index", "_codes", "_scales")
+    MXTensor(buffer, shape) takes the buffer of another one (a contiguous uint8
+    tensor of the shape's size); one on the host is for storage and transport.
+    Copies, pickles and torch.save keep (buffer, shape); torch.load reads them with
+    torch.serialization.safe_globals([MXTensor])."""
+
+    __slots__ = ("_buffer", "_shape", "_bytes")
 
     def __init__(self, buffer, shape):
-        self.buffer, self.shape = buffer, shape
-        self._index = buffer.get_device()
-        self._codes = buffer.data_ptr()  # the scales come behind the codes
-        self._scales = self._codes + buffer.numel() // 17 * 16
+        if not isinstance(buffer, torch.Tensor) or buffer.dtype is not torch.uint8 or (
+                buffer.layout is not torch.strided):
+            raise ValueError("buffer: expected a uint8 tensor, got %s" % (
+                buffer.dtype if isinstance(buffer, torch.Tensor) else type(buffer).__name__))
+        try:
+            rows, cols = (operator.index(n) for n in shape)
+        except (TypeError, ValueError):
+            raise ValueError("shape: expected (rows, cols), got %r" % (shape,)) from None
+        if not (0 <= rows <= _MX_MAX and 0 <= cols <= _MX_MAX):
+            raise ValueError("shape: %d x %d is outside [0, %d]" % (rows, cols, _MX_MAX))
+        self._buffer, self._shape, self._bytes = buffer, (rows, cols), _mx_bytes(rows, cols)
+        if buffer.data_ptr() % 16:
+            raise ValueError("buffer: not 16-byte aligned")
+        _addresses(self)
+
+    def __reduce__(self):
+        return MXTensor, (self._buffer, self._shape)
+
+    buffer = property(lambda self: self._buffer)
+    shape = property(lambda self: self._shape)
 
     @property
     def device(self):
-        return self.buffer.device
+        return self._buffer.device
 
     def dequantize(self, dtype=torch.float32):
         return mx_dequantize(self, dtype)
 
     def __repr__(self):
-        return "MXTensor(%d x %d, %s)" % (self.shape[0], self.shape[1], self.device)
+        return "MXTensor(%d x %d, %s)" % (*self._shape, self.device)
+
+
+def _addresses(q):
+    """(codes, scales) of q where its buffer is now: its storage may have been
+    exchanged or resized since the last call."""
+    b, n = q._buffer, q._bytes
+    if b.numel() != n or not b.is_contiguous():
+        raise ValueError("buffer: expected %d contiguous bytes for %d x %d, got %s of strides %s" % (
+            n, *q._shape, tuple(b.shape), b.stride()))
+    at = b.data_ptr()
+    return at, at + n // 17 * 16  # the scales come behind the codes
 
 
 def _matrix(name, t):
@@ -217,18 +257,19 @@ def _matrix(name, t):
 
 
 def _mx(name, q, cols=None, index=None):
+    """(device ordinal, codes, scales) of q."""
     if not isinstance(q, MXTensor):
         raise ValueError("%s: expected an MXTensor (mx_quantize), got %s" % (name,
                                                                             type(q).__name__))
-    if cols is not None and q.shape[1] != cols:
-        raise ValueError("%s: expected [*, %d], got %s" % (name, cols, q.shape))
-    if index is not None and q._index != index:
+    if cols is not None and q._shape[1] != cols:
+        raise ValueError("%s: expected [*, %d], got %s" % (name, cols, q._shape))
+    codes, scales = _addresses(q)
+    at = q._buffer.get_device()
+    if at < 0:
+        raise ValueError("%s: expected an MXTensor of the GPU, got one on %s" % (name, q.device))
+    if index is not None and at != index:
         raise ValueError("%s is on %s, not with the other operands" % (name, q.device))
-    return q
-
-
-def _mx_bytes(rows, cols):
-    return -(-rows // 64) * -(-cols // 128) * 4352
+    return at, codes, scales
 
 
 def mx_quantize(x):
@@ -240,21 +281,24 @@ def mx_quantize(x):
     NaN as a whole."""
     code = _matrix("x", x)
     (rows, cols), (s0, s1) = x.shape, x.stride()
-    q = MXTensor(x.new_empty(_mx_bytes(rows, cols), dtype=torch.uint8), (rows, cols))
-    _check(lib.ddpg_mx_quantize(q._index, _stream(q._index), code, x.data_ptr(), rows, cols, s0,
-                                s1, q._codes, q._scales))
+    q, index, n = object.__new__(MXTensor), x.get_device(), _mx_bytes(rows, cols)
+    q._buffer, q._shape, q._bytes = x.new_empty(n, dtype=torch.uint8), (rows, cols), n
+    codes = q._buffer.data_ptr()
+    _check(lib.ddpg_mx_quantize(index, _stream(index), code, x.data_ptr(), rows, cols, s0, s1,
+                                codes, codes + n // 17 * 16))
     return q
 
 
 def mx_dequantize(q, dtype=torch.float32):
     """The values q stands for, [rows, cols].  Exact in float32 and bfloat16;
     float16 rounds what lies outside its range."""
-    _mx("q", q)
     if dtype not in _DTYPES:
         raise ValueError("dtype: %s is none of float32, bfloat16, float16" % dtype)
-    out = q.buffer.new_empty(q.shape, dtype=dtype)
-    _check(lib.ddpg_mx_dequantize(q._index, _stream(q._index), q._codes, q._scales, q.shape[0],
-                                  q.shape[1], _DTYPES[dtype], out.data_ptr(), q.shape[1]))
+    index, codes, scales = _mx("q", q)
+    rows, cols = q._shape
+    out = q._buffer.new_empty((rows, cols), dtype=dtype)
+    _check(lib.ddpg_mx_dequantize(index, _stream(index), codes, scales, rows, cols,
+                                  _DTYPES[dtype], out.data_ptr(), cols))
     return out
 
 
@@ -263,14 +307,14 @@ def mx_linear(x, w, bias=None, act=None, dtype=None):
     MXTensor, w [N, K] an MXTensor, bias [N], act None / "elu" / "tanh".  Sums in
     float32; the result is of x's type, or of dtype (float32 if x is an
     MXTensor)."""
-    _mx("w", w)
-    (N, K), index = w.shape, w._index
+    index, w_codes, w_scales = _mx("w", w)
+    N, K = w._shape
     wp, nb = None, 0
     if act not in _ACTS:
         raise ValueError("act: %r is none of None, 'elu', 'tanh'" % (act,))
     if isinstance(x, MXTensor):
-        _mx("x", x, K, index)
-        M, xp, xc, s0, s1, codes, scales = x.shape[0], None, 0, 0, 0, x._codes, x._scales
+        _, codes, scales = _mx("x", x, K, index)
+        M, xp, xc, s0, s1 = x._shape[0], None, 0, 0, 0
         dtype = dtype or torch.float32
     else:
         xc = _matrix("x", x)
@@ -283,7 +327,7 @@ def mx_linear(x, w, bias=None, act=None, dtype=None):
         codes = scales = None
         nb = lib.ddpg_mx_linear_workspace(M, K, N)
         if nb:
-            ws = w.buffer.new_empty(nb)
+            ws = w._buffer.new_empty(nb)
             wp = ws.data_ptr()
         dtype = dtype or x.dtype
     yc = _DTYPES.get(dtype)
@@ -297,10 +341,9 @@ def mx_linear(x, w, bias=None, act=None, dtype=None):
                 N, w.device, tuple(bias.shape), bias.device))
         bias = bias.contiguous()
         bp = bias.data_ptr()
-    y = w.buffer.new_empty((M, N), dtype=dtype)
-    _check(lib.ddpg_mx_linear(index, _stream(index), xc, xp, s0, s1, codes, scales, M, K, w._codes,
-                              w._scales, N, bc, bp, _ACTS[act], yc, y.data_ptr(), N, wp,
-                              nb))
+    y = w._buffer.new_empty((M, N), dtype=dtype)
+    _check(lib.ddpg_mx_linear(index, _stream(index), xc, xp, s0, s1, codes, scales, M, K, w_codes,
+                              w_scales, N, bc, bp, _ACTS[act], yc, y.data_ptr(), N, wp, nb))
     return y
 
 
@@ -313,9 +356,10 @@ def mx_linear_grad(dy, x, w, need=(True, True), bias=True):
     dw are wanted (None otherwise); bias: whether db is."""
     code = _matrix("dy", dy)
     index = dy.get_device()
-    _mx("x", x, None, index)
-    _mx("w", w, x.shape[1], index)
-    (M, K), N = x.shape, w.shape[0]
+    _, x_codes, x_scales = _mx("x", x, None, index)
+    M, K = x._shape
+    _, w_codes, w_scales = _mx("w", w, K, index)
+    N = w._shape[0]
     if dy.shape != (M, N):
         raise ValueError("dy: expected [%d, %d], got %s" % (M, N, tuple(dy.shape)))
     dx = dw = db = pdx = pdw = pdb = None
@@ -330,9 +374,9 @@ def mx_linear_grad(dy, x, w, need=(True, True), bias=True):
         pdb = db.data_ptr()
     nb = lib.ddpg_mx_linear_grad_workspace(code, M, N, K, dx is not None, dw is not None,
                                            db is not None)
-    ws = x.buffer.new_empty(nb)
+    ws = x._buffer.new_empty(nb)
     s0, s1 = dy.stride()
     _check(lib.ddpg_mx_linear_grad(index, _stream(index), code, dy.data_ptr(), s0, s1, M, N, K,
-                                   x._codes, x._scales, w._codes, w._scales, pdx, pdw, pdb,
+                                   x_codes, x_scales, w_codes, w_scales, pdx, pdw, pdb,
                                    ws.data_ptr(), nb))
     return dx, dw, db
