@@ -13,14 +13,15 @@ Each call launches on torch's current stream of the tensors' device and
 returns without waiting; results and workspaces come from torch's allocator, so
 calls may be captured into a graph.  The operators have no autograd formula of
 their own (the learner's gradients are explicit, as ActorNetwork.train's are): a
-tensor that requires grad is refused while grad mode is on.  Arguments of the
-wrong shape, type or device raise ValueError, the library's own refusals
-DDPGError.
+tensor that requires grad is refused while grad mode is on, one with a
+forward-mode tangent always.  Arguments of the wrong shape, type or device raise
+ValueError, the library's own refusals DDPGError.
 """
 import operator
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib
@@ -38,10 +39,17 @@ def _check(rc):
 _stream = torch._C._cuda_getCurrentRawStream
 
 
+def _has_tangent(t):
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def _tensor(name, t):
     """t's dtype code, after the checks every operand shares."""
     if not isinstance(t, torch.Tensor):
         raise ValueError("%s: expected a tensor, got %s" % (name, type(t).__name__))
+    if _has_tangent(t):
+        raise ValueError("%s carries a forward-mode tangent and the operator has no formula for "
+                         "it; pass .detach()" % name)
     if not t.is_cuda:
         raise ValueError("%s: expected a GPU tensor, got one on %s" % (name, t.device))
     code = _DTYPES.get(t.dtype)
@@ -101,7 +109,8 @@ class _List:
             self.ptr = array("Q", [t.data_ptr() for t in src])
             fine = len(index) == 1 and min(index) >= 0 and not (
                 any([t.requires_grad or t.is_neg() for t in src]) if torch.is_grad_enabled()
-                else any(map(torch.Tensor.is_neg, src)))
+                else any(map(torch.Tensor.is_neg, src))) and not (
+                forward_ad._current_level >= 0 and any(map(_has_tangent, src)))
         except (AttributeError, KeyError, TypeError, RuntimeError):
             fine = False
         if not fine:

@@ -44,3 +44,21 @@ def test_a_copy_outlives_the_original(how):
     torch.cuda.synchronize()
     assert torch.equal(ops.mx_linear(x, c), y) and torch.equal(c.dequantize(), v)
     assert torch.equal(ops.mx_linear(ops.mx_quantize(x), c), y)
+
+
+# ---------------------------------------------------------------- tangents
+def test_duals_are_refused_and_their_primals_taken():
+    import torch.autograd.forward_ad as fw
+    t = rnd(40, 40).cuda()
+    q = ops.mx_quantize(t)
+    calls = (lambda x: ops.global_norm([t, x]), lambda x: ops.clip_by_global_norm([x], 1.0)[0][0],
+             lambda x: ops.clip_by_global_norm([t], 1.0, use_norm=x[0, 0])[0][0],
+             lambda x: ops.mx_quantize(x).dequantize(), lambda x: ops.mx_linear(x, q),
+             lambda x: ops.mx_linear(t, q, bias=x[0]), lambda x: ops.mx_linear_grad(x, q, q)[0])
+    for f in calls:
+        want = f(t)
+        with fw.dual_level():
+            d = fw.make_dual(t, torch.ones_like(t))
+            with pytest.raises(ValueError, match="tangent"):
+                f(d)
+            assert torch.equal(f(d.detach()), want) and torch.equal(f(t), want)
