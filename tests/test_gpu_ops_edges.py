@@ -62,3 +62,39 @@ def test_duals_are_refused_and_their_primals_taken():
             with pytest.raises(ValueError, match="tangent"):
                 f(d)
             assert torch.equal(f(d.detach()), want) and torch.equal(f(t), want)
+
+
+# ---------------------------------------------------------------- activations
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [1, 100, 2048, 4096, 8192])  # rows; tiles of 32, 64, 128, 256
+def test_activations_next_to_zero(M, dt):
+    """act(0 + bias) relative to its value.  ELU: x + x^2 p(x) above -0.5, p within
+    2^-26 / 0.64 and five roundings of terms at most 0.27 of the value, one of the whole:
+    2^-23; below, |y| >= 0.39: the exponential's 2^-24, its argument's |x| e^x
+    (2^-24 + 2^-26) and the difference's 2^-25 are under 2^-23 absolute, 2.8 2^-23 of the value.
+    tanh below 0.5 as ELU: 1.5 2^-23; above, where it is at least 0.46, 2.25 2^-23 absolute:
+    5 2^-23 of the value.  Then one rounding to dt."""
+    n = 700 if M < 8192 else 8300
+    small = torch.logspace(-37, -0.302, n // 2, dtype=torch.float64).float()
+    x = torch.cat([-small, small, -torch.linspace(0.4, 0.6, 201), torch.tensor([-0.0, 0.0])])
+    t = x.double()
+    zero = torch.zeros(M, 1, device="cuda")
+    wq = ops.mx_quantize(torch.zeros(len(x), 1, device="cuda"))
+    f = torch.finfo(dt)
+    for act, want, rel in (
+            ("elu", torch.where(t < 0, torch.expm1(t), t),
+             torch.where(t > -0.5, 1.0, 2.8) * 2.0 ** -23 * (t < 0)),
+            ("tanh", torch.tanh(t), torch.where(t.abs() < 0.5, 1.5 * 2.0 ** -23, 5 * 2.0 ** -23))):
+        y = ops.mx_linear(zero, wq, x.cuda(), act, dtype=dt)
+        assert (y == y[0]).all()  # every row, whichever part of a tile it is in
+        err = (y[0].cpu().double() - want).abs()
+        half = 0 if dt is torch.float32 else f.eps / 2 * (1 + 2.0 ** -12)
+        tol = want.abs() * (rel + half) + f.smallest_normal * f.eps
+        assert (err <= tol).all(), (act, x[err > tol][:5], y[0].cpu()[err > tol][:5])
+    # and not finite: the same in every row
+    odd = torch.tensor([float("nan"), float("inf"), -float("inf")] * 3).cuda()
+    wq = ops.mx_quantize(torch.zeros(9, 1, device="cuda"))
+    y = ops.mx_linear(zero, wq, odd, "elu", dtype=dt).cpu()
+    assert y[:, ::3].isnan().all() and (y[:, 1::3] == float("inf")).all() and (y[:, 2::3] == -1).all()
+    y = ops.mx_linear(zero, wq, odd, "tanh", dtype=dt).cpu()
+    assert y[:, ::3].isnan().all() and (y[:, 1::3] == 1).all() and (y[:, 2::3] == -1).all()
