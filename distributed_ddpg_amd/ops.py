@@ -40,14 +40,14 @@ _stream = torch._C._cuda_getCurrentRawStream
 
 
 def _has_tangent(t):
-    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+    return forward_ad.unpack_dual(t).tangent is not None
 
 
 def _tensor(name, t):
     """t's dtype code, after the checks every operand shares."""
     if not isinstance(t, torch.Tensor):
         raise ValueError("%s: expected a tensor, got %s" % (name, type(t).__name__))
-    if _has_tangent(t):
+    if forward_ad._current_level >= 0 and _has_tangent(t):
         raise ValueError("%s carries a forward-mode tangent and the operator has no formula for "
                          "it; pass .detach()" % name)
     if not t.is_cuda:
@@ -212,7 +212,9 @@ class MXTensor:
     Copies, pickles and torch.save keep (buffer, shape); torch.load reads them with
     torch.serialization.safe_globals([MXTensor])."""
 
-    __slots__ = ("_buffer", "_shape", "_bytes")
+    # the buffer as a view of its own, so that what happens to the caller's tensor
+    # (resize_, set_ ..) leaves its size and device; the scales' offset behind the codes
+    __slots__ = ("_buffer", "_shape", "_index", "_at")
 
     def __init__(self, buffer, shape):
         if not isinstance(buffer, torch.Tensor) or buffer.dtype is not torch.uint8 or (
@@ -225,15 +227,21 @@ class MXTensor:
             raise ValueError("shape: expected (rows, cols), got %r" % (shape,)) from None
         if not (0 <= rows <= _MX_MAX and 0 <= cols <= _MX_MAX):
             raise ValueError("shape: %d x %d is outside [0, %d]" % (rows, cols, _MX_MAX))
-        self._buffer, self._shape, self._bytes = buffer, (rows, cols), _mx_bytes(rows, cols)
-        if buffer.data_ptr() % 16:
-            raise ValueError("buffer: not 16-byte aligned")
-        _addresses(self)
+        n = _mx_bytes(rows, cols)
+        if buffer.numel() != n or not buffer.is_contiguous() or buffer.data_ptr() % 16:
+            raise ValueError("buffer: expected %d contiguous bytes, 16-byte aligned, for %d x %d, "
+                             "got %s of strides %s" % (n, rows, cols, tuple(buffer.shape),
+                                                       buffer.stride()))
+        self._set(buffer.view(-1), rows, cols)
+
+    def _set(self, buffer, rows, cols):
+        self._buffer, self._shape = buffer, (rows, cols)
+        self._index, self._at = buffer.get_device(), buffer.numel() // 17 * 16
 
     def __reduce__(self):
         return MXTensor, (self._buffer, self._shape)
 
-    buffer = property(lambda self: self._buffer)
+    buffer = property(lambda self: self._buffer.view(-1))
     shape = property(lambda self: self._shape)
 
     @property
@@ -245,17 +253,6 @@ class MXTensor:
 
     def __repr__(self):
         return "MXTensor(%d x %d, %s)" % (*self._shape, self.device)
-
-
-def _addresses(q):
-    """(codes, scales) of q where its buffer is now: its storage may have been
-    exchanged or resized since the last call."""
-    b, n = q._buffer, q._bytes
-    if b.numel() != n or not b.is_contiguous():
-        raise ValueError("buffer: expected %d contiguous bytes for %d x %d, got %s of strides %s" % (
-            n, *q._shape, tuple(b.shape), b.stride()))
-    at = b.data_ptr()
-    return at, at + n // 17 * 16  # the scales come behind the codes
 
 
 def _matrix(name, t):
@@ -272,13 +269,12 @@ def _mx(name, q, cols=None, index=None):
                                                                             type(q).__name__))
     if cols is not None and q._shape[1] != cols:
         raise ValueError("%s: expected [*, %d], got %s" % (name, cols, q._shape))
-    codes, scales = _addresses(q)
-    at = q._buffer.get_device()
-    if at < 0:
+    if q._index < 0:
         raise ValueError("%s: expected an MXTensor of the GPU, got one on %s" % (name, q.device))
-    if index is not None and at != index:
+    if index is not None and q._index != index:
         raise ValueError("%s is on %s, not with the other operands" % (name, q.device))
-    return at, codes, scales
+    codes = q._buffer.data_ptr()  # where it is now: a storage that grows moves
+    return q._index, codes, codes + q._at
 
 
 def mx_quantize(x):
@@ -290,11 +286,11 @@ def mx_quantize(x):
     NaN as a whole."""
     code = _matrix("x", x)
     (rows, cols), (s0, s1) = x.shape, x.stride()
-    q, index, n = object.__new__(MXTensor), x.get_device(), _mx_bytes(rows, cols)
-    q._buffer, q._shape, q._bytes = x.new_empty(n, dtype=torch.uint8), (rows, cols), n
-    codes = q._buffer.data_ptr()
+    q = object.__new__(MXTensor)
+    q._set(x.new_empty(_mx_bytes(rows, cols), dtype=torch.uint8), rows, cols)
+    index, codes = q._index, q._buffer.data_ptr()
     _check(lib.ddpg_mx_quantize(index, _stream(index), code, x.data_ptr(), rows, cols, s0, s1,
-                                codes, codes + n // 17 * 16))
+                                codes, codes + q._at))
     return q
 
 
