@@ -153,7 +153,7 @@ def run_worker(opt, task_index, env_name, episodes, device):
     critic = nets.CriticNetwork(S, A, opt.critic_lr, opt.tau, actor.get_num_trainable_vars(),
                                 scaler, h1=H1, h2=H2)
     sess = nets.Session(device=device, batch_max=max(opt.batch_size // world, 1), rank=rank,
-                        world=world, grad_clip=opt.grad_clip)
+                        world=world, grad_clip=getattr(opt, "grad_clip", None))
     sess.run(nets.global_variables_initializer(seed=opt.seed))
     actor.set_session(sess)
     critic.set_session(sess)
@@ -174,6 +174,7 @@ def run_worker(opt, task_index, env_name, episodes, device):
     # Flat loop over environment steps: every rank performs exactly one
     # learner update per env step once warm, so the collectives inside the
     # fused step pair up across ranks; the stop decision is agreed by all.
+    act_mx = getattr(opt, "act_mx", False)
     stats = []
     episode, t = 0, 0
     state = env.reset()
@@ -182,9 +183,9 @@ def run_worker(opt, task_index, env_name, episodes, device):
     while True:
         # exploration offset 1/(1 + global_step): global_step is the episode
         # counter restored from the checkpoint (ddpg.py:69, 250)
-        if opt.act_mx and t == 0:
+        if act_mx and t == 0:
             actor.publish_mx()
-        act = actor.predict_mx if opt.act_mx else actor.predict
+        act = actor.predict_mx if act_mx else actor.predict
         a = act(np.reshape(state, (1, S))) + (1.0 / (1.0 + global_step))
         state2, r, done, _ = env.step(a[0])
         replay.add(np.reshape(state, (S,)), np.reshape(a, (A,)), r, done,
