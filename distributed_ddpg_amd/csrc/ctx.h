@@ -432,8 +432,10 @@ enum { ACT_H1, ACT_CAT, ACT_CAT2 };
 // ====================================================================== building blocks
 static const float* P(ddpg_ctx* c, const float* base, const Tensor& t) { return base + t.off; }
 
+// A C entry: f's exceptions as status codes and messages.  A null context (a
+// session that was closed) is refused; entries without one pass nullptr itself.
 template <class F>
-static int guard(ddpg_ctx* c, F&& f) {
+static int guard_as(ddpg_ctx* c, F&& f) {
   try {
     f();
     return DDPG_OK;
@@ -446,6 +448,17 @@ static int guard(ddpg_ctx* c, F&& f) {
     g_err = e.what();
     return DDPG_ENOMEM;
   }
+}
+template <class F>
+static int guard(ddpg_ctx* c, F&& f) {
+  return guard_as(c, [&] {
+    if (!c) throw einval("no context: it was never created, or it was destroyed");
+    f();
+  });
+}
+template <class F>
+static int guard(std::nullptr_t, F&& f) {
+  return guard_as(nullptr, f);
 }
 
 template <class F>
