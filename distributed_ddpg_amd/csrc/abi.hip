@@ -425,7 +425,8 @@ int ddpg_set_grad_clip(ddpg_ctx* c, float actor, float critic) {
     if (!(actor >= 0.f) || !(critic >= 0.f))
       throw einval("gradient clip (%g, %g): norms are numbers >= 0 (0: no clip)", actor, critic);
     if (!c->dclip) {
-      HIP_TRY(hipMalloc(&c->clip_part, clip_factor_workspace()));
+      OnDevice on(c->cfg.device);  // the caller's current device may be another one
+      if (!c->clip_part) HIP_TRY(hipMalloc(&c->clip_part, clip_factor_workspace()));
       HIP_TRY(hipMalloc(&c->dclip, 4 * sizeof(float)));
       c->grad_clip[0] = c->grad_clip[1] = -1.f;  // neither slot is written yet
     }

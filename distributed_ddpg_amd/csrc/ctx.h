@@ -432,6 +432,23 @@ enum { ACT_H1, ACT_CAT, ACT_CAT2 };
 // ====================================================================== building blocks
 static const float* P(ddpg_ctx* c, const float* base, const Tensor& t) { return base + t.off; }
 
+// A device made current for a call's allocations and launches; the caller's is put
+// back.
+struct OnDevice {
+  int prev = -1;
+  explicit OnDevice(int device) {
+    int cur = 0;
+    HIP_TRY(hipGetDevice(&cur));
+    if (cur != device) {
+      HIP_TRY(hipSetDevice(device));
+      prev = cur;
+    }
+  }
+  ~OnDevice() {
+    if (prev >= 0) (void)hipSetDevice(prev);
+  }
+};
+
 // A C entry: f's exceptions as status codes and messages.  A null context (a
 // session that was closed) is refused; entries without one pass nullptr itself.
 template <class F>

@@ -1526,6 +1526,7 @@ int ddpg_soft_update(ddpg_ctx* c, int mask) {
 static void mx_alloc(ddpg_ctx* c, bool train) {
   auto& m = c->mx;
   if (m.w2 && (!train || m.ws)) return;
+  OnDevice on(c->cfg.device);  // the caller's current device may be another one
   auto get = [](auto*& p, size_t bytes) {
     if (p) return;
     void* q = nullptr;

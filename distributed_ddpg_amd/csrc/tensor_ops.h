@@ -16,22 +16,6 @@ inline void check_dtype(const char* what, int dtype) {
     throw einval("%s: dtype %d is none of fp32, bf16, fp16", what, dtype);
 }
 
-// The call's device, current for its launches; the caller's is put back.
-struct OnDevice {
-  int prev = -1;
-  explicit OnDevice(int device) {
-    int cur = 0;
-    HIP_TRY(hipGetDevice(&cur));
-    if (cur != device) {
-      HIP_TRY(hipSetDevice(device));
-      prev = cur;
-    }
-  }
-  ~OnDevice() {
-    if (prev >= 0) (void)hipSetDevice(prev);
-  }
-};
-
 // 16 bytes at any address: the compiler emits the unaligned global access
 struct __attribute__((packed, aligned(2))) U16B {
   uint32_t v[4];
