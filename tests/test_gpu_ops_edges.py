@@ -98,3 +98,67 @@ def test_activations_next_to_zero(M, dt):
     assert y[:, ::3].isnan().all() and (y[:, 1::3] == float("inf")).all() and (y[:, 2::3] == -1).all()
     y = ops.mx_linear(zero, wq, odd, "tanh", dtype=dt).cpu()
     assert y[:, ::3].isnan().all() and (y[:, 1::3] == 1).all() and (y[:, 2::3] == -1).all()
+
+
+# ---------------------------------------------------------------- gradient
+def integers(rows, cols, seed):
+    """Values that MXFP4 holds exactly under a scale of 1."""
+    g = torch.Generator().manual_seed(seed)
+    t = torch.tensor([-4.0, -2.0, -1.0, 1.0, 2.0, 3.0, 4.0, 6.0])[
+        torch.randint(0, 8, (rows, cols), generator=g)]
+    t[:, ::32] = 6.0
+    return t.cuda()
+
+
+# (M, K, N): tile, splits of dX and dW with three planes
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("M,K,N", [(1001, 400, 300),    # 32, 1 and 2
+                                   (513, 257, 1025),    # 32, 2 and 1
+                                   (700, 650, 900),     # 64, 2 and 2
+                                   (30000, 100, 60),    # 64, 1 and 32
+                                   (1100, 900, 1050),   # 128, 2 and 2
+                                   (2000, 1100, 1300),  # 128, 1 and 1
+                                   (8190, 65, 4095),    # 128, 2 and 4
+                                   (20000, 200, 200),   # 128, 1 and 32
+                                   (2050, 2049, 2047),  # 256, 2 and 2
+                                   (4099, 2051, 2040)])  # 256, 1 and 2
+def test_every_plane_of_dy_counts(M, K, N, dt):
+    """dY with at most four values a row (dX) or a column (dW), each 2^j (1 + 2^-9 + 2^-18)
+    (fp16: without the last) -- a bit in every plane -- against integers up to 6: a
+    sum has at most 5 bits above and 18 below the point, so float32 holds all of its
+    partial sums and the results are exact.  A lost plane, or one that meets
+    another depth step's operand, shows."""
+    x, w = integers(M, K, 1), integers(N, K, 2)
+    xq, wq = ops.mx_quantize(x), ops.mx_quantize(w)
+    assert torch.equal(xq.dequantize(), x) and torch.equal(wq.dequantize(), w)
+    v = 1 + 2.0 ** -9 + (2.0 ** -18 if dt is torch.float32 else 0)
+    g = torch.Generator().manual_seed(3)
+    dy = torch.zeros(M, N)
+    for _ in range(4):  # a power of two a row
+        dy[torch.arange(M), torch.randint(0, N, (M,), generator=g)] = v
+    dy = (dy * torch.exp2((torch.arange(M) % 5).float())[:, None]).cuda().to(dt)
+    dx, _, db = ops.mx_linear_grad(dy, xq, wq)
+    assert torch.equal(dx, (dy.double() @ w.double()).to(dt))
+    dy = torch.zeros(N, M)
+    for _ in range(4):
+        dy[torch.arange(N), torch.randint(0, M, (N,), generator=g)] = v
+    dy = (dy * torch.exp2(-(torch.arange(N) % 5).float())[:, None]).t().cuda().to(dt)
+    _, dw, db = ops.mx_linear_grad(dy, xq, wq)
+    assert torch.equal(dw, (dy.double().t() @ x.double()).float())
+    assert torch.equal(db, dy.double().sum(0).float())
+
+
+@pytest.mark.parametrize("e", [-60, -100, -110, -115, -120, -126, -130, -140])
+def test_a_tiny_gradient(e):
+    """float32 dY next to bfloat16's smallest number 2^-133: whole down to 2^-110, below
+    it rounded to a multiple of 2^-133.  The sums are float32's, subnormal ones too."""
+    M, K, N = 9, 70, 33
+    x, w = integers(M, K, 1), integers(N, K, 2)
+    dy = (rnd(M, N, seed=5).double() * 2.0 ** e).float().cuda()
+    dx, dw, db = ops.mx_linear_grad(dy, ops.mx_quantize(x), ops.mx_quantize(w))
+    d = dy.double()
+    for got, want, s, k, m in ((dx, d @ w.double(), d.abs() @ w.double().abs(), N, 6),
+                               (dw, d.t() @ x.double(), d.abs().t() @ x.double().abs(), M, 6),
+                               (db, d.sum(0), d.abs().sum(0), M, 0)):
+        tol = s * (3 * k + 2) * 2.0 ** -23 + k * m * 2.0 ** -134 + (3 * k + 2) * 2.0 ** -149
+        assert ((got.double() - want).abs() <= tol).all()
