@@ -127,8 +127,9 @@ __global__ __launch_bounds__(GN_T) void gn_norm_kernel(const double* part, int n
   }
 }
 
-// y = x * s: the float32 product of a float64 scale, rounded once.  given:
-// the norm to use instead of the partial sums' (use_norm).
+// y = x * s in float64, rounded to float32 and from there to a 16-bit type: off by
+// at most half a step of the type and 2^-24 of the value.  given: the norm to use
+// instead of the partial sums' (use_norm).
 __global__ __launch_bounds__(GN_T) void gn_scale_kernel(GnTable t, const double* part, int np,
                                                         const float* given, float clip,
                                                         float* norm) {

@@ -159,13 +159,14 @@ def global_norm(t_list):
 
 def clip_by_global_norm(t_list, clip_norm, use_norm=None, inplace=False):
     """(list_clipped, norm): each tensor times clip_norm / norm where norm =
-    global_norm(t_list) exceeds clip_norm, unchanged (a copy) otherwise.
+    global_norm(t_list) exceeds clip_norm (a float32), unchanged (a copy) otherwise.
+    The norm enters in float64, also where the returned float32 overflows.
 
     use_norm: a float32 scalar tensor of the same device to use as the norm.
     inplace: write the results into t_list's own tensors (dense, or evenly
     spaced rows; no two may overlap).  None entries stay None.  A NaN norm
     makes every result NaN; an infinite one leaves zeros where the input is finite
-    and NaN elsewhere."""
+    and NaN elsewhere, unless clip_norm is infinite too: then nothing changes."""
     t_list = list(t_list)
     clip_norm = float(clip_norm)
     if not clip_norm >= 0:
@@ -355,10 +356,11 @@ def mx_linear(x, w, bias=None, act=None, dtype=None):
 def mx_linear_grad(dy, x, w, need=(True, True), bias=True):
     """(dx, dw, db) of mx_linear's product x w^T + bias (before act) for dy
     [M, N], with the values the MXTensors x [M, K] and w [N, K] stand for: dx = dy w
-    of dy's type, dw = dy^T x and db = dy's column sums in float32.  The
-    quantisation's own derivative is taken as 1 (straight-through), so dx and dw
-    are the gradients of the matrices that were quantised.  need: whether dx,
-    dw are wanted (None otherwise); bias: whether db is."""
+    of dy's type, dw = dy^T x and db = dy's column sums in float32.  dy may have any
+    strides; adjacent columns are read fastest.  The quantisation's own derivative is
+    taken as 1 (straight-through), so dx and dw are the gradients of the matrices that
+    were quantised.  need: whether dx, dw are wanted (None otherwise); bias:
+    whether db is."""
     code = _matrix("dy", dy)
     index = dy.get_device()
     _, x_codes, x_scales = _mx("x", x, None, index)

@@ -289,8 +289,10 @@ int ddpg_global_norm(int device, void* stream, int n, const int* dtype, const vo
                      size_t ws_bytes, float* norm);
 /* tf.clip_by_global_norm: dst = src * (norm <= clip_norm ? 1 : clip_norm /
  * norm), norm written to *norm; use_norm (device, optional) instead of the
- * list's own norm (ws and norm may then be NULL).  A NaN norm makes every
- * result NaN, an infinite one every finite result 0 and the rest NaN.  dst[i]
+ * list's own norm (ws and norm may then be NULL).  The list's own norm enters in
+ * float64, also where *norm overflows.  A NaN norm makes every result NaN; an
+ * infinite one makes finite elements 0 and the others NaN, unless clip_norm is
+ * INFINITY too, which leaves all as they are.  dst[i]
  * == src[i] clips in place (no two tensors of the list may then overlap); any
  * other dst[i] is dense and overlaps no src. */
 int ddpg_clip_by_global_norm(int device, void* stream, int n, const int* dtype,
@@ -323,8 +325,9 @@ int ddpg_mx_linear(int device, void* stream, int x_dtype, const void* x, int64_t
  * quantised x [M, K] and w [N, K] stand for (straight-through: the quantisation's
  * own derivative is taken as 1): dx [M, K] = dy . w (of type dtype), dw [N, K] =
  * dy^T . x, db [N] = column sums (fp32), all dense.  dy enters exactly (as one,
- * two or three bfloat16 planes), sums are fp32.  Outputs may be NULL; x is read
- * for dw only, w for dx only. */
+ * two or three bfloat16 planes; of fp32, bits below 2^-133 are rounded off in dx and
+ * dw), sums are fp32.  dy is read fastest with adjacent columns.  Outputs may be
+ * NULL; x is read for dw only, w for dx only. */
 size_t ddpg_mx_linear_grad_workspace(int dtype, int64_t M, int64_t N, int64_t K, int dx, int dw,
                                      int db);
 int ddpg_mx_linear_grad(int device, void* stream, int dtype, const void* dy,

@@ -162,3 +162,26 @@ def test_a_tiny_gradient(e):
                                (db, d.sum(0), d.abs().sum(0), M, 0)):
         tol = s * (3 * k + 2) * 2.0 ** -23 + k * m * 2.0 ** -134 + (3 * k + 2) * 2.0 ** -149
         assert ((got.double() - want).abs() <= tol).all()
+
+
+# ---------------------------------------------------------------- clip
+def test_a_norm_outside_float32():
+    """The norm of float32 values can overflow float32, never float64: the clip scales by
+    it all the same.  A norm given as float32 infinity leaves zeros."""
+    x = torch.full((1000,), 3e38).cuda()
+    n = float(x[0].double()) * 1000 ** 0.5
+    out, norm = ops.clip_by_global_norm([x], 1e38)
+    assert torch.isinf(norm)
+    c = float(torch.tensor(1e38, dtype=torch.float32).double())
+    want = float(x[0].double()) * (c / n)
+    assert ((out[0].double() - want).abs() <= want * (2.0 ** -24 + 2.0 ** -50)).all()
+    out, _ = ops.clip_by_global_norm([x], 1e38, use_norm=norm)
+    assert not out[0].any()
+    x[7] = float("inf")
+    out, norm = ops.clip_by_global_norm([x], float("inf"))  # the norm alone
+    assert torch.isinf(norm) and torch.equal(out[0], x)
+    out, norm = ops.clip_by_global_norm([x], 1.0)
+    assert out[0][7].isnan() and not out[0][:7].any() and not out[0][8:].any()
+    x[7] = float("nan")
+    out, norm = ops.clip_by_global_norm([x], float("inf"))
+    assert norm.isnan() and out[0].isnan().all()
