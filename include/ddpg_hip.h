@@ -314,7 +314,8 @@ int ddpg_mx_dequantize(int device, void* stream, const void* codes, const void* 
 /* y [M, N] = act(x [M, K] . w [N, K]^T + bias [N]), w quantised.  x != NULL: x is
  * quantised on the way, in ws (ddpg_mx_linear_workspace bytes, 16-byte aligned; 0
  * where a few rows are quantised inside the product); x == NULL: x_codes /
- * x_scales hold it.  Sums in fp32, one rounding to dtype at the end. */
+ * x_scales hold it.  Sums in fp32, one rounding to dtype at the end; act is within
+ * 2^-21 of its value before it (ELU of a 16-bit result: 2^-15). */
 size_t ddpg_mx_linear_workspace(int64_t M, int64_t K, int64_t N);
 int ddpg_mx_linear(int device, void* stream, int x_dtype, const void* x, int64_t x_row_stride,
                    int64_t x_col_stride, const void* x_codes, const void* x_scales, int64_t M,

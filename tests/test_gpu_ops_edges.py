@@ -73,7 +73,12 @@ def test_activations_next_to_zero(M, dt):
     2^-23; below, |y| >= 0.39: the exponential's 2^-24, its argument's |x| e^x
     (2^-24 + 2^-26) and the difference's 2^-25 are under 2^-23 absolute, 2.8 2^-23 of the value.
     tanh below 0.5 as ELU: 1.5 2^-23; above, where it is at least 0.46, 2.25 2^-23 absolute:
-    5 2^-23 of the value.  Then one rounding to dt."""
+    5 2^-23 of the value.  Then one rounding to dt.
+
+    ELU for 16 bits: the smaller of e^x - 1 + 2^-23, off by at most 1.5 2^-23, and x + x^2 / 2,
+    at most x^2 / 6 (1 + |x|) of the value above it.  The second is the smaller up to
+    |x|^3 / 6 <= 1.5 2^-23, |x| <= 0.0103: 2^-15.7 of the value (roundings 2^-23 of it); behind that the
+    first's 1.5 2^-23 is less of it still."""
     n = 700 if M < 8192 else 8300
     small = torch.logspace(-37, -0.302, n // 2, dtype=torch.float64).float()
     x = torch.cat([-small, small, -torch.linspace(0.4, 0.6, 201), torch.tensor([-0.0, 0.0])])
@@ -83,7 +88,8 @@ def test_activations_next_to_zero(M, dt):
     f = torch.finfo(dt)
     for act, want, rel in (
             ("elu", torch.where(t < 0, torch.expm1(t), t),
-             torch.where(t > -0.5, 1.0, 2.8) * 2.0 ** -23 * (t < 0)),
+             (torch.where(t > -0.5, 1.0, 2.8) * 2.0 ** -23 if dt is torch.float32
+              else 2.0 ** -15.6) * (t < 0)),
             ("tanh", torch.tanh(t), torch.where(t.abs() < 0.5, 1.5 * 2.0 ** -23, 5 * 2.0 ** -23))):
         y = ops.mx_linear(zero, wq, x.cuda(), act, dtype=dt)
         assert (y == y[0]).all()  # every row, whichever part of a tile it is in
