@@ -189,41 +189,45 @@ static void gn_check(const GnList& l) {
   }
 }
 
-// In place: no element may belong to two entries (it would be scaled twice,
-// or by two blocks at once).  Rows of different column ranges of one matrix
-// interleave without touching; anything else that meets is refused.
+// In place: no element may belong to two entries (it would be scaled twice, or by
+// two blocks at once), nor to one and another's input or output.  Rows of
+// different column ranges of one matrix interleave without touching; anything else
+// that meets is refused.
 static void gn_check_disjoint(const GnList& l, const float* use_norm) {
   struct Range {
     uintptr_t lo, hi;
     int i;
+    bool write;
+    int64_t row, pitch;  // bytes; row 0: dense
   };
   std::vector<Range> r;
+  auto add = [&](const void* at, int i, bool write, bool rows) {
+    const int64_t es = elem_size(l.dtype[i]), cols = rows && l.cols ? l.cols[i] : 0;
+    const int64_t n = cols ? l.count[i] / cols : 1, ld = cols ? l.ld[i] : 0;
+    if (write && n > 1 && ld < cols) throw einval("tensor %d overlaps itself", i);
+    const int64_t span = cols ? (n - 1) * ld + cols : l.count[i];
+    const uintptr_t p = (uintptr_t)at;
+    r.push_back({p, p + (uintptr_t)(span * es), i, write, cols * es, ld * es});
+    const uintptr_t u = (uintptr_t)use_norm;  // read while the list is written
+    if (write && u && u + sizeof(float) > r.back().lo && u < r.back().hi)
+      throw einval("use_norm lies in tensor %d, which is clipped in place", i);
+  };
   for (int i = 0; i < l.n; ++i) {
     if (!l.count[i]) continue;
-    const int64_t es = elem_size(l.dtype[i]), cols = l.cols ? l.cols[i] : 0;
-    const uintptr_t p = (uintptr_t)l.dst[i];
-    int64_t span = l.count[i];
-    if (cols) {
-      const int64_t rows = l.count[i] / cols;
-      if (rows > 1 && l.ld[i] < cols) throw einval("tensor %d overlaps itself", i);
-      span = (rows - 1) * l.ld[i] + cols;
-    }
-    r.push_back({p, p + (uintptr_t)(span * es), i});
-    const uintptr_t u = (uintptr_t)use_norm;  // read while the list is written
-    if (u && u + sizeof(float) > r.back().lo && u < r.back().hi)
-      throw einval("use_norm lies in tensor %d, which is clipped in place", i);
+    const bool same = l.src[i] == l.dst[i];
+    add(l.dst[i], i, true, same);  // a destination of its own is dense
+    if (!same) add(l.src[i], i, false, true);
   }
   std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
   for (size_t a = 0; a < r.size(); ++a)
     for (size_t b = a + 1; b < r.size() && r[b].lo < r[a].hi; ++b) {
-      const int i = r[a].i, j = r[b].i;
-      const int64_t ei = elem_size(l.dtype[i]), ej = elem_size(l.dtype[j]);
+      if (!r[a].write && !r[b].write) continue;
       bool apart = false;
-      if (l.cols && l.cols[i] && l.cols[j] && l.ld[i] && l.ld[i] * ei == l.ld[j] * ej) {
-        const uintptr_t pitch = (uintptr_t)(l.ld[i] * ei);
-        const uintptr_t at = (r[b].lo - r[a].lo) % pitch;  // j's row within i's pitch
-        apart = at >= (uintptr_t)(l.cols[i] * ei) && at + (uintptr_t)(l.cols[j] * ej) <= pitch;
+      if (r[a].row && r[b].row && r[a].pitch && r[a].pitch == r[b].pitch) {
+        const int64_t at = (int64_t)((r[b].lo - r[a].lo) % (uintptr_t)r[a].pitch);
+        apart = at >= r[a].row && at + r[b].row <= r[a].pitch;  // b's row within a's pitch
       }
+      const int i = r[a].i, j = r[b].i;
       if (!apart) throw einval("tensors %d and %d overlap", std::min(i, j), std::max(i, j));
     }
 }
