@@ -68,7 +68,8 @@ def _tensor(name, t):
 def _rows(t):
     """(cols, ld) of a tensor whose elements, in its own index order, are rows
     of adjacent elements a fixed distance apart; (0, 0) if it is dense in some
-    index order (the operators do not care which); None if neither."""
+    index order (the operators do not care which); None if neither, or for rows
+    longer than a kernel counts."""
     if t.is_contiguous():
         return 0, 0
     dims = [(st, n) for st, n in zip(t.stride(), t.shape) if n != 1]
@@ -89,7 +90,7 @@ def _rows(t):
     while i >= 0 and dims[i][0] == span:
         span *= dims[i][1]
         i -= 1
-    return (cols, ld) if i < 0 else None
+    return (cols, ld) if i < 0 and cols < 1 << 31 else None
 
 
 class _List:

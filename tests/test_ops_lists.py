@@ -1,10 +1,12 @@
-"""Tensor lists that mix tensors clipped in place with others (no GPU needed: the
-checks come first; a call that passes them ends at a device that is not there)."""
+"""Tensor lists that mix tensors clipped in place with others, and their rows (no GPU
+needed: the checks come first; a call that passes them ends at a device that is not
+there)."""
 import ctypes
 
 import pytest
+import torch
 
-from distributed_ddpg_amd import _lib
+from distributed_ddpg_amd import _lib, ops
 
 L = _lib.lib
 NO_DEVICE = 99
@@ -52,3 +54,10 @@ def test_what_meets_is_refused(other):
         assert rc == (_lib.DDPG_EINVAL if meets else _lib.DDPG_EHIP), L.ddpg_global_error()
         if meets:
             assert b"overlap" in L.ddpg_global_error()
+
+
+def test_rows_longer_than_the_kernels_count():
+    """Such rows go through a dense copy (a meta tensor: nothing is allocated)."""
+    t = torch.empty(2, (1 << 31) + 8, device="meta")
+    assert ops._rows(t[:, :1 << 31]) is None
+    assert ops._rows(t[:, :(1 << 31) - 1]) == ((1 << 31) - 1, (1 << 31) + 8)
