@@ -8,6 +8,7 @@ cd "$ROOT/distributed_ddpg_amd/csrc"
 mkdir -p "$ROOT/build_variants"
 V=$1
 shift
-/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -ffp-contract=off -Wall \
-  -Wno-unused-function -I/opt/rocm/include "$@" gemm.hip step.hip dp.hip replay.hip abi.hip sampler.cpp crc32c.cpp -shared \
+/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -ffp-contract=off \
+  -Xclang -target-feature -Xclang -packed-fp32-ops -Wall \
+  -Wno-unused-function -I/opt/rocm/include "$@" *.hip *.cpp -shared \
   -L/opt/rocm/lib -lrccl -Wl,-soname,libddpg_hip.so -o "$ROOT/build_variants/lib_$V.so"
