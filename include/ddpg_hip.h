@@ -160,9 +160,10 @@ int ddpg_set_scaler(ddpg_ctx* ctx, const double* mean, const double* scale, int 
 
 /* Clip each network's gradient by its global norm between the gradient (after
  * the data-parallel sum) and Adam, in the fused step and the 1:1 train calls: g *
- * min(1, clip / norm), i.e. tf.clip_by_global_norm over compute_gradients'
- * list.  Per network the largest norm; 0 (the default) switches the clip off,
- * INFINITY computes the norm only.  DDPG_*_GRAD returns the clipped gradient. */
+ * min(1, clip / norm) with a float32 factor, i.e. tf.clip_by_global_norm over
+ * compute_gradients' list.  Per network the largest norm; 0 (the default) switches
+ * the clip off, INFINITY computes the norm only.  DDPG_*_GRAD returns the clipped
+ * gradient. */
 int ddpg_set_grad_clip(ddpg_ctx* ctx, float actor, float critic);
 /* The norms (before the clip) of the last update; NaN for a network without a
  * clip.  DDPG_ESTATE if ddpg_set_grad_clip was never called.  Synchronises. */
